@@ -20,6 +20,8 @@ c_int = ctypes.c_int
 c_u32 = ctypes.c_uint32
 c_u64 = ctypes.c_uint64
 c_f = ctypes.c_float
+c_d = ctypes.c_double
+c_i64 = ctypes.c_int64
 c_vp = ctypes.c_void_p
 c_u8p = ctypes.POINTER(ctypes.c_uint8)
 
@@ -99,6 +101,22 @@ _PROTOS: dict[str, list] = {
     "hexlib_b200_matmul_epilogue_ln_rope_fp16": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int,
                                                  c_vp, c_int, c_int, c_int, c_int, c_int,
                                                  c_int, c_vp],
+    "hexlib_b200_quantize_e4m3_fp16": [c_vp, c_vp, c_vp, c_int, c_int, c_vp],
+    "hexlib_b200_quantize_weight_e4m3_fp16": [c_vp, c_vp, c_vp, c_int, c_int, c_vp],
+    "hexlib_b200_dequant_e4m3_fp16": [c_vp, c_vp, c_vp, c_int, c_int, c_vp],
+    "hexlib_b200_matmul_epilogue_e4m3": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int,
+                                         c_int, c_int, c_vp],
+    "hexlib_b200_matmul_epilogue_residual_e4m3": [c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                                  c_int, c_int, c_int, c_int, c_vp],
+    "hexlib_b200_norm_gate_residual_fp16": [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_f,
+                                            c_f, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int,
+                                            c_f, c_vp],
+    "hexlib_b200_norm_gate_residual_e4m3": [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_f,
+                                            c_f, c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int,
+                                            c_int, c_f, c_vp],
+    "hexlib_b200_rope_pos_table": [c_int, c_int, c_d, c_d, c_d, c_d, c_d, c_vp, c_vp],
+    "hexlib_b200_rope_pos_fp16": [c_vp, c_i64, c_vp, c_int, c_vp, c_vp, c_f, c_vp, c_i64, c_int,
+                                  c_int, c_int, c_int, c_int, c_vp],
 }
 
 

@@ -5,6 +5,7 @@
 // launcher the batch dispatcher uses, with one image.
 #include <cuda_runtime.h>
 
+#include <initializer_list>
 #include <mutex>
 
 #include "../../include/hexlib_b200.h"
@@ -43,6 +44,10 @@ int kernels_init_device() {
     if (rc == HEXLIB_B200_OK) rc = quant_kernels_init();
     if (rc == HEXLIB_B200_OK) rc = attention_kernels_init();
     if (rc == HEXLIB_B200_OK) rc = diag_kernels_init();
+    if (rc == HEXLIB_B200_OK) rc = e4m3_kernels_init();
+    if (rc == HEXLIB_B200_OK) rc = gemm_e4m3_kernels_init();
+    if (rc == HEXLIB_B200_OK) rc = edge_kernels_init();
+    if (rc == HEXLIB_B200_OK) rc = rope_pos_kernels_init();
     if (rc != HEXLIB_B200_OK) cudaGetLastError();
     g_dev_status[dev] = rc;
   });
@@ -96,6 +101,10 @@ using hb::kernels_init;
 
 static inline cudaStream_t as_stream(void* s) {
   return reinterpret_cast<cudaStream_t>(s);
+}
+
+static inline bool misaligned(const void* p, uintptr_t n) {
+  return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0;
 }
 
 extern "C" {
@@ -411,6 +420,189 @@ int hexlib_b200_attention_fp16(const void* q, const void* k, const void* v,
     return HEXLIB_B200_ERR_INVAL_PARAMS;
   return hb::launch_attention(q, k, v, ctx, Bn, T, D, scale,
                               hb::default_error_word(), as_stream(stream));
+}
+
+// The operators of a transformer block in 8-bit floating point. Their refusals
+// come before the initialisation, so that a refused call needs no device.
+
+int hexlib_b200_quantize_e4m3_fp16(const void* x, void* codes, void* scales, int R, int K,
+                                   void* stream) {
+  if (R < 0 || K <= 0) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (R == 0) return HEXLIB_B200_OK;
+  if (!x || !codes || !scales || misaligned(x, 2) || misaligned(codes, 16) ||
+      misaligned(scales, 4))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  HB_ENTRY_INIT();
+  return hb::launch_quantize_e4m3(x, codes, scales, R, K, as_stream(stream));
+}
+
+int hexlib_b200_quantize_weight_e4m3_fp16(const void* w, void* codes, void* scales, int K, int N,
+                                          void* stream) {
+  if (K <= 0 || N <= 0 || !w || !codes || !scales || misaligned(w, 2) ||
+      misaligned(codes, 16) || misaligned(scales, 4))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  HB_ENTRY_INIT();
+  return hb::launch_quantize_weight_e4m3(w, codes, scales, K, N, as_stream(stream));
+}
+
+int hexlib_b200_dequant_e4m3_fp16(const void* codes, const void* scales, void* out, int R, int K,
+                                  void* stream) {
+  if (R < 0 || K <= 0) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (R == 0) return HEXLIB_B200_OK;
+  if (!codes || !scales || !out || misaligned(codes, 16) || misaligned(scales, 4) ||
+      misaligned(out, 2))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  HB_ENTRY_INIT();
+  return hb::launch_dequant_e4m3(codes, scales, out, R, K, as_stream(stream));
+}
+
+static int matmul_e4m3(const void* a_codes, const void* a_scales, const void* w_codes,
+                       const void* w_scales, const float* bias, const void* r, void* out, int M,
+                       int K, int N, int act, void* stream) {
+  if (M < 0 || K <= 0 || N <= 0 || act < 0 || act > 2) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (M == 0) return HEXLIB_B200_OK;
+  if (!a_codes || !a_scales || !w_codes || !w_scales || !out || misaligned(a_codes, 16) ||
+      misaligned(a_scales, 4) || misaligned(w_codes, 16) || misaligned(w_scales, 4) ||
+      misaligned(bias, 4) || misaligned(r, 2) || misaligned(out, 2))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  HB_ENTRY_INIT();
+  hb::GemmE4m3Desc g{};
+  g.a = a_codes;
+  g.a_scales = static_cast<const uint32_t*>(a_scales);
+  g.w = w_codes;
+  g.w_scales = static_cast<const uint32_t*>(w_scales);
+  g.bias = bias;
+  g.resid = r;
+  g.out = out;
+  g.M = M;
+  g.K = K;
+  g.N = N;
+  g.act = act;
+  return hb::launch_gemm_e4m3(g, hb::default_error_word(), as_stream(stream));
+}
+
+int hexlib_b200_matmul_epilogue_e4m3(const void* a_codes, const void* a_scales,
+                                     const void* w_codes, const void* w_scales,
+                                     const float* bias, void* out, int M, int K, int N, int act,
+                                     void* stream) {
+  return matmul_e4m3(a_codes, a_scales, w_codes, w_scales, bias, nullptr, out, M, K, N, act,
+                     stream);
+}
+
+int hexlib_b200_matmul_epilogue_residual_e4m3(const void* a_codes, const void* a_scales,
+                                              const void* w_codes, const void* w_scales,
+                                              const float* bias, const void* r, void* out, int M,
+                                              int K, int N, int act, void* stream) {
+  if (M > 0 && !r) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  return matmul_e4m3(a_codes, a_scales, w_codes, w_scales, bias, r, out, M, K, N, act, stream);
+}
+
+static int edge(const hb::EdgeDesc& d, bool e4m3, void* stream) {
+  if (d.R < 0 || d.C <= 0 || (d.norm != HEXLIB_B200_NORM_RMS && d.norm != HEXLIB_B200_NORM_LAYER) ||
+      !(d.eps >= 0.f) || d.gate_act < HEXLIB_B200_GATE_NONE || d.gate_act > HEXLIB_B200_GATE_TANH)
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (d.R == 0) return HEXLIB_B200_OK;
+  if (e4m3 && (!d.h_codes != !d.h_scales)) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  const bool has_h = e4m3 ? d.h_codes != nullptr : d.h != nullptr;
+  if (!d.x || has_h != (d.pre_w != nullptr) || (!d.pre_w && d.pre_b) || (!d.post_w && d.post_b))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (d.y ? !d.x_out : (d.post_w || d.gate || d.x_out || !has_h))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (d.gate ? (d.gate_rows <= 0 || d.R % d.gate_rows != 0) : (d.gate_rows != 0 || d.gate_act != 0))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (misaligned(d.x, 2) || misaligned(d.y, 2) || misaligned(d.x_out, 2) || misaligned(d.h, 2) ||
+      misaligned(d.gate, 2) || misaligned(d.pre_w, 4) || misaligned(d.pre_b, 4) ||
+      misaligned(d.post_w, 4) || misaligned(d.post_b, 4) || misaligned(d.h_codes, 16) ||
+      misaligned(d.h_scales, 4))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  // in place: x_out on x or y, h on y; nothing else shares
+  auto shares = [](const void* p, const void* q) { return p && p == q; };
+  if (shares(d.h, d.x_out) || shares(d.h, d.x) || shares(d.gate, d.x_out) || shares(d.gate, d.h))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (shares(d.h_codes, d.h_scales)) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  for (const void* p : {d.x, d.y, d.gate, static_cast<const void*>(d.x_out)})
+    if (shares(p, d.h_codes) || shares(p, d.h_scales)) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  HB_ENTRY_INIT();
+  return hb::launch_edge(d, as_stream(stream));
+}
+
+static hb::EdgeDesc edge_desc(const void* x, const void* y, const float* post_w,
+                              const float* post_b, const void* gate, int gate_rows, int gate_act,
+                              float x_scale, float y_scale, void* x_out, const float* pre_w,
+                              const float* pre_b, int R, int C, int norm, float eps) {
+  hb::EdgeDesc d{};
+  d.x = x;
+  d.y = y;
+  d.post_w = post_w;
+  d.post_b = post_b;
+  d.gate = gate;
+  d.gate_rows = gate_rows;
+  d.gate_act = gate_act;
+  d.x_scale = x_scale;
+  d.y_scale = y_scale;
+  d.x_out = x_out;
+  d.pre_w = pre_w;
+  d.pre_b = pre_b;
+  d.R = R;
+  d.C = C;
+  d.norm = norm;
+  d.eps = eps;
+  return d;
+}
+
+int hexlib_b200_norm_gate_residual_fp16(const void* x, const void* y, const float* post_w,
+                                        const float* post_b, const void* gate, int gate_rows,
+                                        int gate_act, float x_scale, float y_scale, void* x_out,
+                                        const float* pre_w, const float* pre_b, void* h, int R,
+                                        int C, int norm, float eps, void* stream) {
+  hb::EdgeDesc d = edge_desc(x, y, post_w, post_b, gate, gate_rows, gate_act, x_scale, y_scale,
+                             x_out, pre_w, pre_b, R, C, norm, eps);
+  d.h = h;
+  return edge(d, false, stream);
+}
+
+int hexlib_b200_norm_gate_residual_e4m3(const void* x, const void* y, const float* post_w,
+                                        const float* post_b, const void* gate, int gate_rows,
+                                        int gate_act, float x_scale, float y_scale, void* x_out,
+                                        const float* pre_w, const float* pre_b, void* h_codes,
+                                        void* h_scales, int R, int C, int norm, float eps,
+                                        void* stream) {
+  hb::EdgeDesc d = edge_desc(x, y, post_w, post_b, gate, gate_rows, gate_act, x_scale, y_scale,
+                             x_out, pre_w, pre_b, R, C, norm, eps);
+  d.h_codes = h_codes;
+  d.h_scales = h_scales;
+  return edge(d, true, stream);
+}
+
+int hexlib_b200_rope_pos_fp16(const void* x, int64_t x_stride, const int* positions, int n_axes,
+                              const uint64_t* table, const int* axis, float mscale, void* y,
+                              int64_t y_stride, int T, int H, int D, int rot, int layout,
+                              void* stream) {
+  if (T < 0 || H <= 0 || D <= 0 || rot <= 0 || (rot & 1) || rot > D || n_axes < 1 || n_axes > 4 ||
+      (layout != HEXLIB_B200_ROPE_HALF && layout != HEXLIB_B200_ROPE_INTERLEAVED) ||
+      x_stride < (int64_t)H * D || y_stride < (int64_t)H * D)
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (T == 0) return HEXLIB_B200_OK;
+  if (!x || !y || !positions || !table || (x == y && x_stride != y_stride) || misaligned(x, 2) ||
+      misaligned(y, 2) || misaligned(positions, 4) || misaligned(table, 8) || misaligned(axis, 4))
+    return HEXLIB_B200_ERR_INVAL_PARAMS;
+  HB_ENTRY_INIT();
+  hb::RopePosDesc d{};
+  d.x = x;
+  d.x_stride = x_stride;
+  d.positions = positions;
+  d.n_axes = n_axes;
+  d.table = table;
+  d.axis = axis;
+  d.mscale = mscale;
+  d.y = y;
+  d.y_stride = y_stride;
+  d.T = T;
+  d.H = H;
+  d.D = D;
+  d.rot = rot;
+  d.layout = layout;
+  return hb::launch_rope_pos(d, as_stream(stream));
 }
 
 int hexlib_b200_stream_status(void* stream) {

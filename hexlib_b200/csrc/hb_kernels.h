@@ -139,6 +139,68 @@ int launch_attention(const void* q, const void* k, const void* v, void* ctx,
 int launch_attention_qkv(const void* qkv, void* ctx, int64_t B, int T, int H, int D,
                          float scale, int* err, cudaStream_t s);
 
+// 8-bit floating point (k_e4m3.cu, k_gemm_e4m3.cu). The e4m3 form of R rows of
+// K: codes [R, Kp] and scale bytes [ceil(Kp / 512), R, 4], Kp = e4m3_pitch(K).
+inline int64_t e4m3_pitch(int64_t K) { return (K + 127) / 128 * 128; }
+inline int64_t e4m3_scale_groups(int64_t K) { return (K + 511) / 512; }
+int e4m3_kernels_init();
+int launch_quantize_e4m3(const void* x, void* codes, void* scales, int64_t R, int K,
+                         cudaStream_t s);
+// of the transpose of w [K, N]
+int launch_quantize_weight_e4m3(const void* w, void* codes, void* scales, int K, int N,
+                                cudaStream_t s);
+int launch_dequant_e4m3(const void* codes, const void* scales, void* out, int64_t R, int K,
+                        cudaStream_t s);
+struct GemmE4m3Desc {
+  const void* a;            // codes of M rows of K
+  const uint32_t* a_scales; // words of 4 scale bytes, [ceil(K / 512), M]
+  const void* w;            // codes of N rows of K
+  const uint32_t* w_scales;
+  const float* bias;        // [N] or nullptr
+  const void* resid;        // [M, N] fp16 or nullptr
+  void* out;                // [M, N] fp16
+  int M, K, N, act;
+};
+int gemm_e4m3_kernels_init();
+int launch_gemm_e4m3(const GemmE4m3Desc& g, int* err, cudaStream_t s);
+
+// The edge between two blocks (k_edge.cu); h or h_codes + h_scales, or neither.
+struct EdgeDesc {
+  const void* x;
+  const void* y;            // nullptr: x' = x
+  const float* post_w;      // nullptr: u = y
+  const float* post_b;
+  const void* gate;         // [gate_rows, C] or nullptr
+  int gate_rows, gate_act;
+  float x_scale, y_scale;
+  void* x_out;
+  const float* pre_w;
+  const float* pre_b;
+  void* h;
+  void* h_codes;
+  void* h_scales;
+  int R, C, norm;
+  float eps;
+};
+int edge_kernels_init();
+int launch_edge(const EdgeDesc& d, cudaStream_t s);
+
+// Rotary positions (k_rope_pos.cu).
+struct RopePosDesc {
+  const void* x;
+  int64_t x_stride;
+  const int* positions;     // [n_axes, T]
+  int n_axes;
+  const uint64_t* table;    // [rot / 2] turns per position, times 2^64
+  const int* axis;          // [rot / 2] or nullptr
+  float mscale;
+  void* y;
+  int64_t y_stride;
+  int T, H, D, rot, layout;
+};
+int rope_pos_kernels_init();
+int launch_rope_pos(const RopePosDesc& d, cudaStream_t s);
+
 // Diagnostic: a kernel whose bounded wait never completes; it records a
 // timeout in `err` after `limit_us` and returns.
 int launch_wait_timeout_probe(int* err, uint32_t limit_us, cudaStream_t s);

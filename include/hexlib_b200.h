@@ -374,6 +374,121 @@ HEXLIB_B200_API int hexlib_b200_attention_fp16(const void *q, const void *k, con
                                void *ctx, int Bn, int T, int D, float scale,
                                void *stream);
 
+/* ---- 8-bit floating point, block edges, rotary positions -------------------
+ * The operators of a language model's transformer block next to the encoder's
+ * kernels above (no counterpart in the reference, whose weights are q4_0 and
+ * whose only rotation is rope_2d). All of them take an empty batch (no rows, no
+ * tokens) and then launch nothing, are ordered on `stream`, allocate nothing and
+ * may be captured into a CUDA graph. `stream` must belong to the current device. */
+
+/* THE E4M3 FORM of a matrix of R rows of K fp16 values. A row is cut into blocks
+ * of 128 (the last one padded with zeros). A block's scale is the power of two
+ * 2^e with the smallest integer e for which every finite |x| <= 448 * 2^e (e = 0
+ * for a block of zeros), its codes are x * 2^-e rounded to nearest even; the
+ * product is exact, so a value is rounded once. Infinities and NaN become NaN
+ * codes and do not enter the scale.
+ *   codes   uint8 [R, Kp], Kp = K rounded up to 128; the padding is 0
+ *   scales  uint8 [ceil(Kp / 512), R, 4]: the byte e + 127 of block b of row r
+ *           at ((b / 4) * R + r) * 4 + b % 4; the padding is 127
+ * codes must be 16-byte aligned, scales 4-byte. */
+#define HEXLIB_B200_E4M3_BLOCK 128
+HEXLIB_B200_API int hexlib_b200_quantize_e4m3_fp16(const void *x, void *codes, void *scales,
+                                                   int R, int K, void *stream);
+/* The e4m3 form of the TRANSPOSE of a [K, N] row-major fp16 weight: N rows of K,
+ * the operand hexlib_b200_matmul_epilogue_e4m3 takes. Done once per weight. */
+HEXLIB_B200_API int hexlib_b200_quantize_weight_e4m3_fp16(const void *w, void *codes,
+                                                          void *scales, int K, int N,
+                                                          void *stream);
+/* The values an e4m3 form stands for, rounded to fp16: out [R, K]. (A code times
+ * its scale is exact in fp16 but for magnitudes under 2^-15, which may round, and
+ * 65536, which is infinite there.) */
+HEXLIB_B200_API int hexlib_b200_dequant_e4m3_fp16(const void *codes, const void *scales,
+                                                  void *out, int R, int K, void *stream);
+/* out[M, N] = act(a @ w + bias), rounded once to fp16: a the e4m3 form of M rows
+ * of K, w that of the [K, N] weight (N rows of K), fp32 sums, act as in
+ * hexlib_b200_matmul_epilogue_fp16. bias may be NULL. Neither operand is
+ * dequantized: codes and scales go to the tensor cores. */
+HEXLIB_B200_API int hexlib_b200_matmul_epilogue_e4m3(const void *a_codes, const void *a_scales,
+                                                     const void *w_codes, const void *w_scales,
+                                                     const float *bias, void *out, int M, int K,
+                                                     int N, int act, void *stream);
+/* The same plus a residual r [M, N] fp16: out = act(a @ w + bias) + r, rounded
+ * once. out may be r. */
+HEXLIB_B200_API int hexlib_b200_matmul_epilogue_residual_e4m3(
+    const void *a_codes, const void *a_scales, const void *w_codes, const void *w_scales,
+    const float *bias, const void *r, void *out, int M, int K, int N, int act, void *stream);
+
+/* THE EDGE BETWEEN TWO BLOCKS, over R rows of C: the norm after a block, its gate
+ * and residual scale, and the norm before the next block, in one pass:
+ *   u  = norm(y; post_w, post_b), or y when post_w is NULL
+ *   x' = fp16(x_scale * x + y_scale * f(gate[r / (R / gate_rows)]) * u)
+ *   h  = fp16(norm(x'; pre_w, pre_b))
+ * norm is v / sqrt(mean(v^2) + eps) * w (+ b) for HEXLIB_B200_NORM_RMS and
+ * (v - mean) / sqrt(var + eps) * w (+ b) for HEXLIB_B200_NORM_LAYER; w and b are
+ * fp32 [C], b may be NULL. gate is fp16 [gate_rows, C]: 1 row for a per-channel
+ * gate, one for each image or sequence, or R of them; gate_rows must divide R.
+ * gate NULL (gate_rows 0) means 1. h is the norm of the stored x'.
+ * pre_w NULL with h NULL: x' alone. y NULL (with post_w, gate and x_out NULL):
+ * x' = x, h alone -- the norm before the first block.
+ * In place: x_out may be x or y, and h may be y. Every other overlap is refused
+ * where the pointers are equal and undefined where they are not. */
+#define HEXLIB_B200_NORM_RMS     0
+#define HEXLIB_B200_NORM_LAYER   1
+#define HEXLIB_B200_GATE_NONE    0   /* f(g) = g           */
+#define HEXLIB_B200_GATE_SIGMOID 1
+#define HEXLIB_B200_GATE_SILU    2   /* f(g) = g sigmoid(g) */
+#define HEXLIB_B200_GATE_TANH    3
+HEXLIB_B200_API int hexlib_b200_norm_gate_residual_fp16(
+    const void *x, const void *y, const float *post_w, const float *post_b, const void *gate,
+    int gate_rows, int gate_act, float x_scale, float y_scale, void *x_out, const float *pre_w,
+    const float *pre_b, void *h, int R, int C, int norm, float eps, void *stream);
+/* The same with h in its e4m3 form: exactly hexlib_b200_quantize_e4m3_fp16 of the
+ * h above, without writing and reading it. h_codes and h_scales overlap nothing. */
+HEXLIB_B200_API int hexlib_b200_norm_gate_residual_e4m3(
+    const void *x, const void *y, const float *post_w, const float *post_b, const void *gate,
+    int gate_rows, int gate_act, float x_scale, float y_scale, void *x_out, const float *pre_w,
+    const float *pre_b, void *h_codes, void *h_scales, int R, int C, int norm, float eps,
+    void *stream);
+
+/* ROTARY POSITIONS. Pair j of the first `rot` elements of a head turns by
+ * positions[axis[j]][t] * table[j] / 2^64 turns: the table is in 64-bit fixed
+ * point, so the product modulo 2^64 is the exact phase at any int32 position,
+ * however far. y = mscale * (a cos - b sin, a sin + b cos), fp32, rounded once. */
+#define HEXLIB_B200_ROPE_HALF        0   /* pair j: elements j and j + rot / 2   */
+#define HEXLIB_B200_ROPE_INTERLEAVED 1   /* pair j: elements 2j and 2j + 1       */
+#define HEXLIB_B200_ROPE_SCALE_NONE   0
+#define HEXLIB_B200_ROPE_SCALE_LINEAR 1  /* positions divided by `factor`        */
+#define HEXLIB_B200_ROPE_SCALE_BASE   2  /* theta * factor^(rot / (rot - 2))      */
+#define HEXLIB_B200_ROPE_SCALE_YARN   3
+#define HEXLIB_B200_ROPE_SCALE_BANDED 4
+/* Fill the HOST array table[rot / 2] and *mscale from theta and a scaling for
+ * contexts longer than `length` (a host function: no device, no stream). The
+ * plain frequency of pair j is f = theta^(-2j / rot) radians per position.
+ *   YARN    f / factor where f turns fewer than `low` times in `length`
+ *           positions, f where it turns more than `high` times, a ramp over the
+ *           pairs between (from the floor of the pair that turns `high` times to
+ *           the ceiling of the one that turns `low` times); mscale = 1 + 0.1
+ *           ln(factor) for factor > 1
+ *   BANDED  the same bands, blended by the number of turns itself; mscale = 1
+ * factor, length, low, high are read only by the scalings that use them and must
+ * then be finite and positive, with low < high. theta > 1; rot even. */
+HEXLIB_B200_API int hexlib_b200_rope_pos_table(int scaling, int rot, double theta, double factor,
+                                               double length, double low, double high,
+                                               uint64_t *table, float *mscale);
+/* Rotate the first H heads of D of every token: x row t starts at x + t * x_stride
+ * elements, y row t at y + t * y_stride (strides >= H * D), so q and k of a packed
+ * projection are rotated in one call, in place when y is x and the strides are
+ * equal. Elements from rot on are copied. positions is int32 [n_axes, T] (1 to 4
+ * axes: text, or time, height and width), axis int32 [rot / 2] on the device,
+ * clamped to [0, n_axes), NULL for axis 0 everywhere. Negative positions turn
+ * back: the call with negated positions is the gradient of the rotation and undoes
+ * it (up to mscale^2). */
+HEXLIB_B200_API int hexlib_b200_rope_pos_fp16(const void *x, int64_t x_stride,
+                                              const int *positions, int n_axes,
+                                              const uint64_t *table, const int *axis,
+                                              float mscale, void *y, int64_t y_stride, int T,
+                                              int H, int D, int rot, int layout, void *stream);
+
 /* ---- the embedding gather across GPUs (NCCL, with deadlines) --------------
  * The image-sharded encoder's one exchange: an all-gather of every rank's fp16
  * embeddings. No counterpart in the reference, which runs one image at a time
