@@ -150,6 +150,12 @@ __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   return a;
 }
 
+__device__ __forceinline__ float ld_cluster_f32(uint32_t caddr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(caddr) : "memory");
+  return v;
+}
+
 __device__ __forceinline__ void st_cluster_u32(uint32_t caddr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(caddr), "r"(v) : "memory");
 }
@@ -239,6 +245,15 @@ __device__ __forceinline__ void tma_load_3d(const CUtensorMap* map,
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* bar,
+                                            void* smem_dst, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+      : "memory");
+}
+
 // Bulk tensor store shared::cta -> global, tracked by bulk async-groups.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map,
                                              const void* smem_src, int c0,
@@ -321,6 +336,29 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem,
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accum)
       : "memory");
+}
+
+// D[tmem] (+)= A * B for e4m3 operands with a power-of-two scale for every 32 of K:
+// `sfa` / `sfb` address the scale bytes in tensor memory (row r of the operand: lane
+// r % 32 of column r / 32, repeated in the four lane quarters; idesc picks one of the
+// word's four bytes). K = 32, issued by one thread.
+__device__ __forceinline__ void umma_e4m3_scaled(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                                 uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                                 uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X "
+      "[%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accum)
+      : "memory");
+}
+
+// Copy 32 rows of 16 bytes from shared memory to four columns of tensor memory,
+// the same in each lane quarter. Ordered before later tcgen05.mma of the thread.
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc)
+               : "memory");
 }
 
 // Arrive once on `bar` when every tcgen05.mma this thread issued so far has
@@ -416,6 +454,16 @@ __device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr,
       : "memory");
 }
 
+// 32 lanes x 8 consecutive fp32 columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+
 // 32 lanes x 16 consecutive fp32 columns, register -> TMEM.
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr,
                                                    const uint32_t (&r)[16]) {
@@ -465,6 +513,26 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr, uint32_t lbo,
   d |= static_cast<uint64_t>(1) << 46;
   d |= static_cast<uint64_t>(2) << 61;
   return d;
+}
+
+// Descriptor of 32 rows of 16 contiguous bytes, unswizzled: 8-row groups 128 bytes
+// apart (SBO), one 16-byte column (LBO unused).
+__device__ __forceinline__ uint64_t sdesc_rows16(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128u >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  return d;
+}
+
+// Instruction descriptor for kind::mxf8f6f4 with e4m3 operands, both K-major, E8M0
+// scales, fp32 D: [4,6) B's scale byte, [7,10) A format (0 = e4m3), [10,13) B format,
+// [17,23) N>>3, [23] scale format (1 = E8M0), [24,29) M>>4, [29,31) A's scale byte.
+__host__ __device__ constexpr uint32_t idesc_e4m3_scaled(uint32_t M, uint32_t N) {
+  return ((N >> 3) << 17) | (1u << 23) | ((M >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t idesc_with_scale_byte(uint32_t idesc, uint32_t i) {
+  return idesc | (i << 4) | (i << 29);
 }
 
 // Instruction descriptor for kind::f16: fp16 A and B, fp32 D, dense.

@@ -63,4 +63,20 @@ bool make_tmap_3d_f16(CUtensorMap* map, const void* base, uint64_t x,
                                   box_y);
 }
 
+bool make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t x, uint64_t y,
+                     uint32_t box_y) {
+  if (!tma_available()) return false;
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || x == 0 || y == 0 || x % 16 ||
+      box_y == 0 || box_y > 256)
+    return false;
+  const cuuint64_t dims[2] = {x, y};
+  const cuuint64_t strides[1] = {x};
+  const cuuint32_t box[2] = {128, box_y};
+  const cuuint32_t estr[2] = {1, 1};
+  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides,
+                  box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace hb

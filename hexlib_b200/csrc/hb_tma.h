@@ -27,4 +27,10 @@ bool make_tmap_3d_f16_strided(CUtensorMap* map, const void* base, uint64_t x,
                               uint64_t pitch_z, uint32_t box_x,
                               uint32_t box_y);
 
+// Tensor map over a row-major [y, x] byte array: box (128, box_y), 128-byte
+// swizzle, out-of-range rows filled with zeros. `base` 16-byte aligned, x a
+// multiple of 16.
+bool make_tmap_2d_u8(CUtensorMap* map, const void* base, uint64_t x, uint64_t y,
+                     uint32_t box_y);
+
 }  // namespace hb
