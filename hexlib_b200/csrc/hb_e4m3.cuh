@@ -46,6 +46,97 @@ __device__ __forceinline__ float e4m3_value(uint32_t code) {
       __half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
 }
 
+// The codes of a block of 128 fp16 values held by 16 consecutive lanes (half of a
+// warp, the lanes of `half_mask`), 8 to a lane as four words of two, and the block's
+// scale byte. The largest magnitude is found on the bits (halves of the same sign
+// order as integers), two to an instruction.
+__device__ __forceinline__ uint2 e4m3_encode8(const uint32_t (&w)[4], uint32_t half_mask,
+                                              uint32_t& byte) {
+  uint32_t m2 = w[0] & 0x7fff7fffu;
+#pragma unroll
+  for (int j = 1; j < 4; ++j) m2 = __vmaxu2(m2, w[j] & 0x7fff7fffu);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m2 = __vmaxu2(m2, __shfl_xor_sync(half_mask, m2, o));
+  uint32_t m = max(m2 & 0xffffu, m2 >> 16);
+  const bool finite = m < 0x7c00u;
+  if (!finite) {                       // the same for all 16 lanes
+    m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int h = 0; h < 32; h += 16) {
+        const uint32_t a = (w[j] >> h) & 0x7fffu;
+        if (a < 0x7c00u) m = max(m, a);
+      }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(half_mask, m, o));
+  }
+  byte = e4m3_scale_byte(__half2float(__ushort_as_half((unsigned short)m)));
+  const float inv = e4m3_inverse(byte);
+  uint32_t c[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+    c[j] = finite ? e4m3_pack2(__fmul_rn(f.x, inv), __fmul_rn(f.y, inv))
+                  : e4m3_code(f.x, inv) | (e4m3_code(f.y, inv) << 8);
+  }
+  return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+}
+
+// Eight fp16 values from p, as four words of two, in loads of VEC values (VEC = 8 for
+// 16-byte aligned rows down to 1 for any); values from `left` on are zeros. With
+// VEC > 1, `left` is a multiple of VEC.
+template <int VEC>
+__device__ __forceinline__ void load8(uint32_t (&w)[4], const __half* p, int left) {
+  if constexpr (VEC == 8) {
+    const uint4 u = left > 0 ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  } else if constexpr (VEC == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const uint2 u = 2 * j < left ? *reinterpret_cast<const uint2*>(p + 2 * j) : make_uint2(0, 0);
+      w[j] = u.x; w[j + 1] = u.y;
+    }
+  } else if constexpr (VEC == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = 2 * j < left ? *reinterpret_cast<const uint32_t*>(p + 2 * j) : 0u;
+  } else {
+    const unsigned short* q = reinterpret_cast<const unsigned short*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      w[j] = (2 * j < left ? (uint32_t)q[2 * j] : 0u) |
+             (2 * j + 1 < left ? (uint32_t)q[2 * j + 1] << 16 : 0u);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void store8(__half* p, const uint32_t (&w)[4], int left) {
+  if constexpr (VEC == 8) {
+    if (left > 0) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else if constexpr (VEC == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; j += 2)
+      if (2 * j < left) *reinterpret_cast<uint2*>(p + 2 * j) = make_uint2(w[j], w[j + 1]);
+  } else if constexpr (VEC == 2) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (2 * j < left) *reinterpret_cast<uint32_t*>(p + 2 * j) = w[j];
+  } else {
+    unsigned short* q = reinterpret_cast<unsigned short*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (2 * j < left) q[2 * j] = (unsigned short)w[j];
+      if (2 * j + 1 < left) q[2 * j + 1] = (unsigned short)(w[j] >> 16);
+    }
+  }
+}
+// The widest VEC of rows of C values starting at p (and at q).
+inline int row_vec(int64_t C, const void* p, const void* q = nullptr) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) |
+                      static_cast<uintptr_t>(2 * C);
+  return a % 16 == 0 ? 8 : a % 8 == 0 ? 4 : a % 4 == 0 ? 2 : 1;
+}
+
 // Byte offset of the scale of block b of row r of R.
 __device__ __forceinline__ int64_t e4m3_scale_at(int64_t r, int b, int64_t R) {
   return ((b >> 2) * R + r) * 4 + (b & 3);

@@ -15,38 +15,76 @@ int grid_for(int64_t items) {
   return static_cast<int>(blocks < 148 * 8 ? blocks : 148 * 8);
 }
 
-// One warp per block of 128 values; the value i of row r is x[r * sr + i * si], so
-// the same kernel reads a matrix and its transpose. Blocks past the row's last
-// (up to a whole word of scales) only get their scale byte.
-__global__ void quantize_e4m3(const __half* __restrict__ x, uint8_t* __restrict__ codes,
-                              uint8_t* __restrict__ scales, int64_t R, int K, int64_t sr,
-                              int64_t si) {
-  const int lane = threadIdx.x & 31;
+// Half a warp per scale word: 512 values of a row, a block of 128 at a time, 8 to a
+// lane, so a lane has four 16-byte loads in flight and a word is stored whole. Bound
+// by memory: 2 bytes read and 1 written per value.
+template <int VEC>
+__global__ void __launch_bounds__(kThreads) quantize_e4m3(const __half* __restrict__ x,
+                                                          uint8_t* __restrict__ codes,
+                                                          uint32_t* __restrict__ scales,
+                                                          int64_t R, int K) {
+  const int l = threadIdx.x & 15;
+  const uint32_t half_mask = 0xffffu << (threadIdx.x & 16);
+  const int blocks = (K + 127) / 128, groups = (blocks + 3) / 4;
+  const int64_t t = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 4;
+  if (t >= R * groups) return;
+  const int64_t r = t / groups;
+  const int g = (int)(t - r * groups);
+  uint32_t w[4][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k = g * 512 + j * 128 + l * 8;
+    load8<VEC>(w[j], x + r * K + k, K - k);
+  }
+  uint32_t word = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k = g * 512 + j * 128 + l * 8;
+    uint32_t byte;
+    const uint2 c = e4m3_encode8(w[j], half_mask, byte);
+    if (g * 4 + j < blocks)
+      *reinterpret_cast<uint2*>(codes + r * (int64_t)blocks * 128 + k) = c;
+    word |= byte << (8 * j);           // (a block past the last is zeros: 1.0)
+  }
+  if (l == 0) scales[(int64_t)g * R + r] = word;
+}
+
+// The form of the transpose of w [K, N]: a CTA turns a block of 128 of K by 32 columns
+// through shared memory, then a warp has a column's block, 4 values to a lane. Done
+// once per weight.
+__global__ void __launch_bounds__(kThreads) quantize_weight_e4m3(const __half* __restrict__ w,
+                                                                 uint8_t* __restrict__ codes,
+                                                                 uint8_t* __restrict__ scales,
+                                                                 int K, int N) {
+  __shared__ __half tile[128][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int blocks = (K + 127) / 128, padded = (blocks + 3) / 4 * 4;
-  const int64_t pitch = blocks * 128;
-  const int64_t total = R * padded;
-  for (int64_t t = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5; t < total;
-       t += ((int64_t)gridDim.x * blockDim.x) >> 5) {
-    const int64_t r = t / padded;
-    const int b = (int)(t - r * padded);
-    uint32_t byte = kE4m3One;
-    if (b < blocks) {
-      float v[4], amax = 0.f;
+  const int n_tiles = (N + 31) / 32;
+  const int b = blockIdx.x / n_tiles, n0 = (blockIdx.x % n_tiles) * 32;
+  for (int i = warp; i < 128; i += kThreads / 32) {
+    const int64_t k = (int64_t)b * 128 + i;
+    tile[i][lane] = k < K && n0 + lane < N ? w[k * N + n0 + lane] : __half(0.f);
+  }
+  __syncthreads();
+  for (int c = warp; c < 32 && n0 + c < N; c += kThreads / 32) {
+    const int64_t n = n0 + c;
+    float v[4], amax = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int k = b * 128 + lane + 32 * j;
-        v[j] = k < K ? __half2float(x[r * sr + k * si]) : 0.f;
-        if (isfinite(v[j])) amax = fmaxf(amax, fabsf(v[j]));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      byte = e4m3_scale_byte(amax);
-      const float inv = e4m3_inverse(byte);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        codes[r * pitch + b * 128 + lane + 32 * j] = (uint8_t)e4m3_code(v[j], inv);
+    for (int j = 0; j < 4; ++j) {
+      v[j] = __half2float(tile[lane * 4 + j][c]);
+      if (isfinite(v[j])) amax = fmaxf(amax, fabsf(v[j]));
     }
-    if (lane == 0) scales[e4m3_scale_at(r, b, R)] = (uint8_t)byte;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const uint32_t byte = e4m3_scale_byte(amax);
+    const float inv = e4m3_inverse(byte);
+    uint32_t q = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) q |= e4m3_code(v[j], inv) << (8 * j);
+    *reinterpret_cast<uint32_t*>(codes + n * (int64_t)blocks * 128 + b * 128 + lane * 4) = q;
+    if (lane == 0) scales[e4m3_scale_at(n, b, N)] = (uint8_t)byte;
+    if (b == blocks - 1 && lane < padded - blocks)
+      scales[e4m3_scale_at(n, blocks + lane, N)] = (uint8_t)kE4m3One;
   }
 }
 
@@ -76,7 +114,9 @@ int launched() {
 // Load the kernels now, so that none is loaded lazily inside a graph capture.
 int e4m3_kernels_init() {
   cudaFuncAttributes a;
-  for (const void* f : {(const void*)quantize_e4m3, (const void*)dequant_e4m3})
+  for (const void* f : {(const void*)quantize_e4m3<8>, (const void*)quantize_e4m3<4>,
+                        (const void*)quantize_e4m3<2>, (const void*)quantize_e4m3<1>,
+                        (const void*)quantize_weight_e4m3, (const void*)dequant_e4m3})
     if (cudaFuncGetAttributes(&a, f) != cudaSuccess) {
       cudaGetLastError();
       return HEXLIB_B200_ERR_CUDA;
@@ -86,15 +126,27 @@ int e4m3_kernels_init() {
 
 int launch_quantize_e4m3(const void* x, void* codes, void* scales, int64_t R, int K,
                          cudaStream_t s) {
-  quantize_e4m3<<<grid_for(R * e4m3_scale_groups(K) * 4 * 32), kThreads, 0, s>>>(
-      (const __half*)x, (uint8_t*)codes, (uint8_t*)scales, R, K, K, 1);
-  return launched();
+  const int64_t ctas = (R * e4m3_scale_groups(K) * 16 + kThreads - 1) / kThreads;
+  if (ctas > 0x7fffffff) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  auto go = [&](auto kernel) {
+    kernel<<<(unsigned)ctas, kThreads, 0, s>>>((const __half*)x, (uint8_t*)codes,
+                                               (uint32_t*)scales, R, K);
+    return launched();
+  };
+  switch (row_vec(K, x)) {
+    case 8: return go(quantize_e4m3<8>);
+    case 4: return go(quantize_e4m3<4>);
+    case 2: return go(quantize_e4m3<2>);
+  }
+  return go(quantize_e4m3<1>);
 }
 
 int launch_quantize_weight_e4m3(const void* w, void* codes, void* scales, int K, int N,
                                 cudaStream_t s) {
-  quantize_e4m3<<<grid_for(N * e4m3_scale_groups(K) * 4 * 32), kThreads, 0, s>>>(
-      (const __half*)w, (uint8_t*)codes, (uint8_t*)scales, N, K, 1, N);
+  const int64_t ctas = e4m3_pitch(K) / 128 * ((N + 31) / 32);
+  if (ctas > 0x7fffffff) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  quantize_weight_e4m3<<<(unsigned)ctas, kThreads, 0, s>>>((const __half*)w, (uint8_t*)codes,
+                                                           (uint8_t*)scales, K, N);
   return launched();
 }
 
