@@ -1,8 +1,12 @@
 // k_edge.cu -- the edge between two transformer blocks in one pass over the rows:
 //   u  = norm(y) (or y);  x' = fp16(x_scale x + y_scale f(gate) u);
 //   h  = fp16(norm(x')), or that in its e4m3 form (hb_e4m3.cuh).
+// Bound by memory: 4 bytes read and 4 (3 with 8-bit h) written per value, 2 more
+// where the gate has a row of its own for every row.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "hb_e4m3.cuh"
 #include "hb_kernels.h"
@@ -14,135 +18,342 @@ constexpr int kThreads = 256;
 
 __device__ __forceinline__ float gate_value(float g, int act) {
   switch (act) {
-    case HEXLIB_B200_GATE_SIGMOID: return 1.f / (1.f + expf(-g));
-    case HEXLIB_B200_GATE_SILU: return g / (1.f + expf(-g));
+    case HEXLIB_B200_GATE_SIGMOID: return __fdividef(1.f, 1.f + expf(-g));
+    case HEXLIB_B200_GATE_SILU: return __fdividef(g, 1.f + expf(-g));
     case HEXLIB_B200_GATE_TANH: return tanhf(g);
   }
   return g;
 }
 
-// One value of a norm, every rounding written out: the fp16 and the 8-bit form (and
-// every row layout) then give the same bits from the same moments.
-__device__ __forceinline__ float normed(float v, float2 ms, float w, const float* b, int c) {
+// One value of a norm, every rounding written out: the fp16 and the 8-bit form then
+// give the same bits from the same moments.
+__device__ __forceinline__ float normed(float v, float2 ms, float w, bool has_b, float b) {
   v = __fmul_rn(__fsub_rn(v, ms.x), ms.y);
-  return b ? fmaf(v, w, b[c]) : __fmul_rn(v, w);
+  return has_b ? fmaf(v, w, b) : __fmul_rn(v, w);
 }
-__device__ __forceinline__ __half blended(float x_scale, float x, float y_scale, float u) {
-  return __float2half_rn(fmaf(x_scale, x, __fmul_rn(y_scale, u)));
+__device__ __forceinline__ float blended(float x_scale, float x, float y_scale, float u) {
+  return fmaf(x_scale, x, __fmul_rn(y_scale, u));
 }
 
-__device__ __forceinline__ float cta_sum(float v, float* red) {
+// Sum over the G threads of a row: a warp, or the CTA through shared memory. The
+// slots rotate, so that one barrier a sum suffices: a slot is written again only
+// three barriers after it was read.
+template <int G>
+struct RowSum {
+  float (*red)[kThreads / 32];
+  int slot = 0;
+  __device__ float operator()(float v) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.f;
-  for (int i = 0; i < kThreads / 32; ++i) t += red[i];
-  __syncthreads();
-  return t;
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (G == 32) return v;
+    float* r = red[slot];
+    slot = (slot + 1) & 3;
+    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < G / 32; ++i) t += r[i];
+    return t;
+  }
+};
+
+__device__ __forceinline__ float2 halves(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <int VEC>
+__device__ __forceinline__ void load8f(float (&f)[8], const float* p, int left) {
+  if constexpr (VEC == 8) {
+    const float4 a = left > 0 ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
+    const float4 b = left > 0 ? __ldg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = i < left ? __ldg(p + i) : 0.f;
+  }
 }
 
-// mean (0 for rms) and 1 / sqrt(mean of squared deviations + eps) of a row
-__device__ __forceinline__ float2 moments(const __half* v, int C, bool layer, float eps,
-                                          float* red) {
+// mean (0 for rms) and 1 / sqrt(mean squared deviation + eps) of a row of C values in
+// registers: vector j of thread g at column (j G + g) 8, zeros past C.
+template <int G, int V>
+__device__ __forceinline__ float2 moments(const uint32_t (&w)[V][4], int g, int C, bool layer,
+                                          float eps, RowSum<G>& sum) {
+  float mean = 0.f;
+  if (layer) {
+    float s = 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 f = halves(w[j][q]);
+        s += f.x + f.y;
+      }
+    mean = sum(s) / C;
+  }
+  float ss = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int left = C - (j * G + g) * 8;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 f = halves(w[j][q]);
+      const float a = 2 * q < left ? f.x - mean : 0.f, b = 2 * q + 1 < left ? f.y - mean : 0.f;
+      ss = fmaf(a, a, fmaf(b, b, ss));
+    }
+  }
+  return make_float2(mean, 1.f / sqrtf(sum(ss) / C + eps));
+}
+
+// A row of up to G * V * 8 values in the registers of G threads (a warp, or the CTA),
+// read once and written once.
+template <int G, int V, int VEC, bool E4M3>
+__global__ void __launch_bounds__(kThreads) edge_held(const EdgeDesc d) {
+  __shared__ float red[4][kThreads / 32];
+  RowSum<G> sum{red};
+  const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
+  const int g = G == 32 ? (threadIdx.x & 31) : threadIdx.x;
+  const int per_gate = d.gate ? d.R / d.gate_rows : 1;
+  const int C = d.C, blocks = (C + 127) / 128, padded = (blocks + 3) / 4 * 4;
+  const int64_t first = G == 32 ? blockIdx.x * (int64_t)(kThreads / 32) + (threadIdx.x >> 5)
+                                : (int64_t)blockIdx.x;
+  const int64_t step = G == 32 ? (int64_t)gridDim.x * (kThreads / 32) : (int64_t)gridDim.x;
+  for (int64_t r = first; r < d.R; r += step) {
+    uint32_t x[V][4];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (j * G + g) * 8;
+      load8<VEC>(x[j], (const __half*)d.x + r * C + c, C - c);
+    }
+    if (d.y) {
+      uint32_t y[V][4];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = (j * G + g) * 8;
+        load8<VEC>(y[j], (const __half*)d.y + r * C + c, C - c);
+      }
+      float2 ms = make_float2(0.f, 1.f);
+      if (d.post_w) ms = moments<G, V>(y, g, C, layer, d.eps, sum);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = (j * G + g) * 8;
+        float u[8];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 f = halves(y[j][q]);
+          u[2 * q] = f.x;
+          u[2 * q + 1] = f.y;
+        }
+        if (d.post_w) {
+          float w[8], b[8];
+          load8f<VEC>(w, d.post_w + c, C - c);
+          if (d.post_b) load8f<VEC>(b, d.post_b + c, C - c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) u[i] = normed(u[i], ms, w[i], d.post_b != nullptr, b[i]);
+        }
+        if (d.gate) {
+          uint32_t w[4];
+          load8<VEC>(w, (const __half*)d.gate + (r / per_gate) * C + c, C - c);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 f = halves(w[q]);
+            u[2 * q] = __fmul_rn(u[2 * q], gate_value(f.x, d.gate_act));
+            u[2 * q + 1] = __fmul_rn(u[2 * q + 1], gate_value(f.y, d.gate_act));
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float2 f = halves(x[j][q]);
+          const bool in0 = 2 * q < C - c, in1 = 2 * q + 1 < C - c;   // zeros stay past C
+          x[j][q] = pack(in0 ? blended(d.x_scale, f.x, d.y_scale, u[2 * q]) : 0.f,
+                         in1 ? blended(d.x_scale, f.y, d.y_scale, u[2 * q + 1]) : 0.f);
+        }
+        store8<VEC>((__half*)d.x_out + r * C + c, x[j], C - c);
+      }
+    }
+    if (!d.pre_w) continue;
+    const float2 ms = moments<G, V>(x, g, C, layer, d.eps, sum);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = (j * G + g) * 8;
+      float w[8], b[8];
+      load8f<VEC>(w, d.pre_w + c, C - c);
+      if (d.pre_b) load8f<VEC>(b, d.pre_b + c, C - c);
+      uint32_t h[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 f = halves(x[j][q]);
+        const bool in0 = 2 * q < C - c, in1 = 2 * q + 1 < C - c;
+        h[q] = pack(in0 ? normed(f.x, ms, w[2 * q], d.pre_b != nullptr, b[2 * q]) : 0.f,
+                    in1 ? normed(f.y, ms, w[2 * q + 1], d.pre_b != nullptr, b[2 * q + 1]) : 0.f);
+      }
+      if constexpr (!E4M3) {
+        store8<VEC>((__half*)d.h + r * C + c, h, C - c);
+      } else {
+        // 16 consecutive threads hold a block; blocks past the last are zeros
+        const int b128 = c >> 7;
+        uint32_t byte;
+        const uint2 codes = e4m3_encode8(h, 0xffffu << (threadIdx.x & 16), byte);
+        if (b128 < blocks)
+          *reinterpret_cast<uint2*>((uint8_t*)d.h_codes + r * (int64_t)blocks * 128 + c) = codes;
+        if ((threadIdx.x & 15) == 0 && b128 < padded)
+          ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b128, d.R)] = (uint8_t)byte;
+      }
+    }
+    if constexpr (E4M3) {
+      // scale bytes of the last word that no thread's columns reach
+      for (int b = G * V / 16 + g; b < padded; b += G)
+        ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b, d.R)] = (uint8_t)kE4m3One;
+    }
+  }
+}
+
+// Rows wider than the registers hold: one CTA per row, read again for each pass. A
+// thread reads x' of other threads' columns only after the barriers of the sums.
+__device__ __forceinline__ float2 moments_wide(const __half* v, int C, bool layer, float eps,
+                                               RowSum<kThreads>& sum) {
   float mean = 0.f;
   if (layer) {
     float s = 0.f;
     for (int c = threadIdx.x; c < C; c += kThreads) s += __half2float(v[c]);
-    mean = cta_sum(s, red) / C;
+    mean = sum(s) / C;
   }
   float ss = 0.f;
   for (int c = threadIdx.x; c < C; c += kThreads) {
     const float d = __half2float(v[c]) - mean;
     ss = fmaf(d, d, ss);
   }
-  return make_float2(mean, 1.f / sqrtf(cta_sum(ss, red) / C + eps));
+  return make_float2(mean, 1.f / sqrtf(sum(ss) / C + eps));
 }
 
-// One CTA per row, its values read again from global memory for each pass; a thread
-// reads x' back only where it wrote it, and the sums between the passes order them.
 template <bool E4M3>
-__global__ void __launch_bounds__(kThreads) edge_rows(const EdgeDesc d) {
-  __shared__ float red[kThreads / 32];
+__global__ void __launch_bounds__(kThreads) edge_wide(const EdgeDesc d) {
+  __shared__ float red[4][kThreads / 32];
+  RowSum<kThreads> sum{red};
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
   const int per_gate = d.gate ? d.R / d.gate_rows : 1;
   for (int64_t r = blockIdx.x; r < d.R; r += gridDim.x) {
     const __half* x = (const __half*)d.x + r * d.C;
     if (d.y) {
       const __half* y = (const __half*)d.y + r * d.C;
+      const __half* gate = (const __half*)d.gate + (r / per_gate) * d.C;
       __half* xo = (__half*)d.x_out + r * d.C;
       float2 ms = make_float2(0.f, 1.f);
-      if (d.post_w) ms = moments(y, d.C, layer, d.eps, red);
+      if (d.post_w) ms = moments_wide(y, d.C, layer, d.eps, sum);
       for (int c = threadIdx.x; c < d.C; c += kThreads) {
         float u = __half2float(y[c]);
-        if (d.post_w) u = normed(u, ms, d.post_w[c], d.post_b, c);
-        if (d.gate)
-          u = __fmul_rn(u, gate_value(__half2float(((const __half*)d.gate)[(r / per_gate) * d.C + c]),
-                                      d.gate_act));
-        xo[c] = blended(d.x_scale, __half2float(x[c]), d.y_scale, u);
+        if (d.post_w) u = normed(u, ms, d.post_w[c], d.post_b, d.post_b ? d.post_b[c] : 0.f);
+        if (d.gate) u = __fmul_rn(u, gate_value(__half2float(gate[c]), d.gate_act));
+        xo[c] = __float2half_rn(blended(d.x_scale, __half2float(x[c]), d.y_scale, u));
       }
       x = xo;
     }
     if (!d.pre_w) continue;
-    const float2 ms = moments(x, d.C, layer, d.eps, red);
+    const float2 ms = moments_wide(x, d.C, layer, d.eps, sum);
     auto h_of = [&](int c) {
-      return __float2half_rn(normed(__half2float(x[c]), ms, d.pre_w[c], d.pre_b, c));
+      return __float2half_rn(normed(__half2float(x[c]), ms, d.pre_w[c], d.pre_b,
+                                    d.pre_b ? d.pre_b[c] : 0.f));
     };
     if constexpr (!E4M3) {
       for (int c = threadIdx.x; c < d.C; c += kThreads) ((__half*)d.h)[r * d.C + c] = h_of(c);
     } else {
-      // a warp per block of 128; the x' of other threads' columns is visible after
-      // the barriers inside moments()
-      const int blocks = (d.C + 127) / 128, padded = (blocks + 3) / 4 * 4, lane = threadIdx.x & 31;
-      uint8_t* codes = (uint8_t*)d.h_codes + r * (int64_t)blocks * 128;
-      for (int b = threadIdx.x >> 5; b < padded; b += kThreads / 32) {
-        uint32_t byte = kE4m3One;
-        if (b < blocks) {
-          float v[4], amax = 0.f;
+      const int blocks = (d.C + 127) / 128, padded = (blocks + 3) / 4 * 4;
+      const int l = threadIdx.x & 15;
+      for (int b0 = 0; b0 < padded; b0 += kThreads / 16) {
+        const int b = b0 + (threadIdx.x >> 4), c = b * 128 + l * 8;
+        uint32_t h[4], byte;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int c = b * 128 + lane + 32 * j;
-            v[j] = c < d.C ? __half2float(h_of(c)) : 0.f;
-            if (isfinite(v[j])) amax = fmaxf(amax, fabsf(v[j]));
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1)
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-          byte = e4m3_scale_byte(amax);
-          const float inv = e4m3_inverse(byte);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            codes[b * 128 + lane + 32 * j] = (uint8_t)e4m3_code(v[j], inv);
+        for (int q = 0; q < 4; ++q) {
+          const __half lo = c + 2 * q < d.C ? h_of(c + 2 * q) : __half(0.f);
+          const __half hi = c + 2 * q + 1 < d.C ? h_of(c + 2 * q + 1) : __half(0.f);
+          h[q] = __half_as_ushort(lo) | ((uint32_t)__half_as_ushort(hi) << 16);
         }
-        if (lane == 0) ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b, d.R)] = (uint8_t)byte;
+        const uint2 codes = e4m3_encode8(h, 0xffffu << (threadIdx.x & 16), byte);
+        if (b < blocks)
+          *reinterpret_cast<uint2*>((uint8_t*)d.h_codes + r * (int64_t)blocks * 128 + c) = codes;
+        if (l == 0 && b < padded)
+          ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b, d.R)] = (uint8_t)byte;
       }
     }
   }
 }
 
-}  // namespace
+// Every (threads per row, vectors per thread) a width can take.
+template <class F>
+int with_layout(int C, F&& f) {
+  const int v = (C + 7) / 8;
+#define HB_EDGE_LAYOUT(G, V) \
+  if (v <= G * V) return f(std::integral_constant<int, G>{}, std::integral_constant<int, V>{});
+  HB_EDGE_LAYOUT(32, 1)
+  HB_EDGE_LAYOUT(32, 2)
+  HB_EDGE_LAYOUT(32, 3)
+  HB_EDGE_LAYOUT(32, 4)
+  HB_EDGE_LAYOUT(256, 1)
+  HB_EDGE_LAYOUT(256, 2)
+  HB_EDGE_LAYOUT(256, 3)
+  HB_EDGE_LAYOUT(256, 4)
+  HB_EDGE_LAYOUT(256, 8)
+#undef HB_EDGE_LAYOUT
+  return f(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
+}
 
-int edge_kernels_init() {
-  cudaFuncAttributes a;
-  for (const void* f : {(const void*)edge_rows<false>, (const void*)edge_rows<true>})
-    if (cudaFuncGetAttributes(&a, f) != cudaSuccess) {
+template <int VEC, bool E4M3>
+int launch_form(const EdgeDesc& d, cudaStream_t s) {
+  return with_layout(d.C, [&](auto G, auto V) {
+    if constexpr (G.value == 0) {
+      edge_wide<E4M3><<<d.R < 148 * 8 ? d.R : 148 * 8, kThreads, 0, s>>>(d);
+    } else {
+      const int64_t rows = G.value == 32 ? kThreads / 32 : 1;
+      const int64_t ctas = (d.R + rows - 1) / rows;
+      edge_held<G.value, V.value, VEC, E4M3>
+          <<<(unsigned)(ctas < 148 * 8 ? ctas : 148 * 8), kThreads, 0, s>>>(d);
+    }
+    if (cudaPeekAtLastError() != cudaSuccess) {
       cudaGetLastError();
       return HEXLIB_B200_ERR_CUDA;
     }
-  return HEXLIB_B200_OK;
+    return HEXLIB_B200_OK;
+  });
 }
 
-int launch_edge(const EdgeDesc& d, cudaStream_t s) {
-  const int grid = d.R < 148 * 8 ? d.R : 148 * 8;
-  if (d.h_codes)
-    edge_rows<true><<<grid, kThreads, 0, s>>>(d);
-  else
-    edge_rows<false><<<grid, kThreads, 0, s>>>(d);
-  if (cudaPeekAtLastError() != cudaSuccess) {
+template <int VEC, bool E4M3>
+bool load_form() {
+  cudaFuncAttributes a;
+  bool ok = cudaFuncGetAttributes(&a, (const void*)edge_wide<E4M3>) == cudaSuccess;
+  for (int C : {256, 512, 768, 1024, 2048, 4096, 6144, 8192, 16384})
+    with_layout(C, [&](auto G, auto V) {
+      if constexpr (G.value != 0)
+        ok = ok && cudaFuncGetAttributes(
+                       &a, (const void*)edge_held<G.value, V.value, VEC, E4M3>) == cudaSuccess;
+      return 0;
+    });
+  return ok;
+}
+
+}  // namespace
+
+// Load the kernels now, so that none is loaded lazily inside a graph capture.
+int edge_kernels_init() {
+  if (!load_form<8, false>() || !load_form<8, true>() || !load_form<1, false>() ||
+      !load_form<1, true>()) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
   return HEXLIB_B200_OK;
+}
+
+int launch_edge(const EdgeDesc& d, cudaStream_t s) {
+  uintptr_t bits = static_cast<uintptr_t>(2) * d.C;
+  for (const void* p : {d.x, d.y, d.gate, (const void*)d.x_out, (const void*)d.h,
+                        (const void*)d.pre_w, (const void*)d.pre_b, (const void*)d.post_w,
+                        (const void*)d.post_b})
+    bits |= reinterpret_cast<uintptr_t>(p);
+  const bool wide = bits % 16 == 0;
+  if (d.h_codes) return wide ? launch_form<8, true>(d, s) : launch_form<1, true>(d, s);
+  return wide ? launch_form<8, false>(d, s) : launch_form<1, false>(d, s);
 }
 
 }  // namespace hb
