@@ -74,11 +74,22 @@ __device__ __forceinline__ uint2 e4m3_encode8(const uint32_t (&w)[4], uint32_t h
   byte = e4m3_scale_byte(__half2float(__ushort_as_half((unsigned short)m)));
   const float inv = e4m3_inverse(byte);
   uint32_t c[4];
+  if (finite && byte >= 112u) {
+    // 2^-e fits fp16, and the product in fp16 loses only bits of values under 2^-14,
+    // which e4m3 rounds to zero all the same (its smallest step is 2^-9)
+    const __half2 inv2 = __half2half2(__float2half_rn(inv));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-    c[j] = finite ? e4m3_pack2(__fmul_rn(f.x, inv), __fmul_rn(f.y, inv))
-                  : e4m3_code(f.x, inv) | (e4m3_code(f.y, inv) << 8);
+    for (int j = 0; j < 4; ++j)
+      c[j] = __nv_cvt_halfraw2_to_fp8x2(
+          __half2_raw(__hmul2(*reinterpret_cast<const __half2*>(&w[j]), inv2)), __NV_SATFINITE,
+          __NV_E4M3);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      c[j] = finite ? e4m3_pack2(__fmul_rn(f.x, inv), __fmul_rn(f.y, inv))
+                    : e4m3_code(f.x, inv) | (e4m3_code(f.y, inv) << 8);
+    }
   }
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }

@@ -25,8 +25,21 @@ __device__ __forceinline__ float gate_value(float g, int act) {
   return g;
 }
 
-// One value of a norm, every rounding written out: the fp16 and the 8-bit form then
-// give the same bits from the same moments.
+// The gate's function of a pair, its branch taken once for eight values.
+__device__ __forceinline__ void gate_values(float2 (&g)[4], int act) {
+  if (act == HEXLIB_B200_GATE_NONE) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) g[q] = make_float2(gate_value(g[q].x, act), gate_value(g[q].y, act));
+}
+
+// A pair of a norm's values, every rounding written out (two-wide instructions round
+// both as the scalar ones do): every form gives the same bits from the same moments.
+// `shift` is minus the mean.
+__device__ __forceinline__ float2 normed2(float2 v, float shift, float inv, float2 w, bool has_b,
+                                          float2 b) {
+  v = __fmul2_rn(__fadd2_rn(v, make_float2(shift, shift)), make_float2(inv, inv));
+  return has_b ? __ffma2_rn(v, w, b) : __fmul2_rn(v, w);
+}
 __device__ __forceinline__ float normed(float v, float2 ms, float w, bool has_b, float b) {
   v = __fmul_rn(__fsub_rn(v, ms.x), ms.y);
   return has_b ? fmaf(v, w, b) : __fmul_rn(v, w);
@@ -65,53 +78,64 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <int VEC>
-__device__ __forceinline__ void load8f(float (&f)[8], const float* p, int left) {
+__device__ __forceinline__ void load8f(float2 (&f)[4], const float* p, int left) {
   if constexpr (VEC == 8) {
     const float4 a = left > 0 ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
     const float4 b = left > 0 ? __ldg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+    f[0] = make_float2(a.x, a.y);
+    f[1] = make_float2(a.z, a.w);
+    f[2] = make_float2(b.x, b.y);
+    f[3] = make_float2(b.z, b.w);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < left ? __ldg(p + i) : 0.f;
+    for (int q = 0; q < 4; ++q)
+      f[q] = make_float2(2 * q < left ? __ldg(p + 2 * q) : 0.f,
+                         2 * q + 1 < left ? __ldg(p + 2 * q + 1) : 0.f);
   }
+}
+// Zeros from `left` on (a multiple of 8 when VEC is 8, so the whole vector or nothing).
+template <int VEC>
+__device__ __forceinline__ uint32_t pack_in(float2 f, int q, int left) {
+  if constexpr (VEC == 8) return left > 0 ? pack(f.x, f.y) : 0u;
+  return pack(2 * q < left ? f.x : 0.f, 2 * q + 1 < left ? f.y : 0.f);
 }
 
 // mean (0 for rms) and 1 / sqrt(mean squared deviation + eps) of a row of C values in
 // registers: vector j of thread g at column (j G + g) 8, zeros past C.
-template <int G, int V>
+template <int G, int V, int VEC>
 __device__ __forceinline__ float2 moments(const uint32_t (&w)[V][4], int g, int C, bool layer,
                                           float eps, RowSum<G>& sum) {
   float mean = 0.f;
   if (layer) {
-    float s = 0.f;
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 f = halves(w[j][q]);
-        s += f.x + f.y;
-      }
-    mean = sum(s) / C;
+      for (int q = 0; q < 4; ++q) s = __fadd2_rn(s, halves(w[j][q]));
+    mean = sum(s.x + s.y) / C;
   }
-  float ss = 0.f;
+  const float2 shift = make_float2(-mean, -mean);
+  float2 ss = make_float2(0.f, 0.f);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int left = C - (j * G + g) * 8;
+    if (VEC == 8 && left <= 0) continue;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float2 f = halves(w[j][q]);
-      const float a = 2 * q < left ? f.x - mean : 0.f, b = 2 * q + 1 < left ? f.y - mean : 0.f;
-      ss = fmaf(a, a, fmaf(b, b, ss));
+      float2 f = __fadd2_rn(halves(w[j][q]), shift);
+      if (VEC != 8 && 2 * q >= left) f.x = 0.f;
+      if (VEC != 8 && 2 * q + 1 >= left) f.y = 0.f;
+      ss = __ffma2_rn(f, f, ss);
     }
   }
-  return make_float2(mean, 1.f / sqrtf(sum(ss) / C + eps));
+  return make_float2(mean, 1.f / sqrtf(sum(ss.x + ss.y) / C + eps));
 }
 
 // A row of up to G * V * 8 values in the registers of G threads (a warp, or the CTA),
-// read once and written once.
+// read once and written once; its gate is read with it, ahead of the sums.
 template <int G, int V, int VEC, bool E4M3>
-__global__ void __launch_bounds__(kThreads) edge_held(const EdgeDesc d) {
+__global__ void __launch_bounds__(kThreads, V == 1 ? 4 : V <= 3 ? 3 : V == 4 ? 2 : 1)
+    edge_held(const EdgeDesc d) {
   __shared__ float red[4][kThreads / 32];
   RowSum<G> sum{red};
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
@@ -129,67 +153,63 @@ __global__ void __launch_bounds__(kThreads) edge_held(const EdgeDesc d) {
       load8<VEC>(x[j], (const __half*)d.x + r * C + c, C - c);
     }
     if (d.y) {
-      uint32_t y[V][4];
+      uint32_t y[V][4], gate[V][4];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int c = (j * G + g) * 8;
         load8<VEC>(y[j], (const __half*)d.y + r * C + c, C - c);
       }
+      if (d.gate) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int c = (j * G + g) * 8;
+          load8<VEC>(gate[j], (const __half*)d.gate + (r / per_gate) * C + c, C - c);
+        }
+      }
       float2 ms = make_float2(0.f, 1.f);
-      if (d.post_w) ms = moments<G, V>(y, g, C, layer, d.eps, sum);
+      if (d.post_w) ms = moments<G, V, VEC>(y, g, C, layer, d.eps, sum);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int c = (j * G + g) * 8;
-        float u[8];
+        float2 u[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float2 f = halves(y[j][q]);
-          u[2 * q] = f.x;
-          u[2 * q + 1] = f.y;
-        }
+        for (int q = 0; q < 4; ++q) u[q] = halves(y[j][q]);
         if (d.post_w) {
-          float w[8], b[8];
+          float2 w[4], b[4];
           load8f<VEC>(w, d.post_w + c, C - c);
           if (d.post_b) load8f<VEC>(b, d.post_b + c, C - c);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) u[i] = normed(u[i], ms, w[i], d.post_b != nullptr, b[i]);
+          for (int q = 0; q < 4; ++q)
+            u[q] = normed2(u[q], -ms.x, ms.y, w[q], d.post_b != nullptr, b[q]);
         }
         if (d.gate) {
-          uint32_t w[4];
-          load8<VEC>(w, (const __half*)d.gate + (r / per_gate) * C + c, C - c);
+          float2 f[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float2 f = halves(w[q]);
-            u[2 * q] = __fmul_rn(u[2 * q], gate_value(f.x, d.gate_act));
-            u[2 * q + 1] = __fmul_rn(u[2 * q + 1], gate_value(f.y, d.gate_act));
-          }
-        }
+          for (int q = 0; q < 4; ++q) f[q] = halves(gate[j][q]);
+          gate_values(f, d.gate_act);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float2 f = halves(x[j][q]);
-          const bool in0 = 2 * q < C - c, in1 = 2 * q + 1 < C - c;   // zeros stay past C
-          x[j][q] = pack(in0 ? blended(d.x_scale, f.x, d.y_scale, u[2 * q]) : 0.f,
-                         in1 ? blended(d.x_scale, f.y, d.y_scale, u[2 * q + 1]) : 0.f);
+          for (int q = 0; q < 4; ++q) u[q] = __fmul2_rn(u[q], f[q]);
         }
+        const float2 xs = make_float2(d.x_scale, d.x_scale), ys = make_float2(d.y_scale, d.y_scale);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          x[j][q] = pack_in<VEC>(__ffma2_rn(xs, halves(x[j][q]), __fmul2_rn(ys, u[q])), q, C - c);
         store8<VEC>((__half*)d.x_out + r * C + c, x[j], C - c);
       }
     }
     if (!d.pre_w) continue;
-    const float2 ms = moments<G, V>(x, g, C, layer, d.eps, sum);
+    const float2 ms = moments<G, V, VEC>(x, g, C, layer, d.eps, sum);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (j * G + g) * 8;
-      float w[8], b[8];
+      float2 w[4], b[4];
       load8f<VEC>(w, d.pre_w + c, C - c);
       if (d.pre_b) load8f<VEC>(b, d.pre_b + c, C - c);
       uint32_t h[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 f = halves(x[j][q]);
-        const bool in0 = 2 * q < C - c, in1 = 2 * q + 1 < C - c;
-        h[q] = pack(in0 ? normed(f.x, ms, w[2 * q], d.pre_b != nullptr, b[2 * q]) : 0.f,
-                    in1 ? normed(f.y, ms, w[2 * q + 1], d.pre_b != nullptr, b[2 * q + 1]) : 0.f);
-      }
+      for (int q = 0; q < 4; ++q)
+        h[q] = pack_in<VEC>(normed2(halves(x[j][q]), -ms.x, ms.y, w[q], d.pre_b != nullptr, b[q]),
+                            q, C - c);
       if constexpr (!E4M3) {
         store8<VEC>((__half*)d.h + r * C + c, h, C - c);
       } else {
