@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "hb_e4m3.cuh"
@@ -16,20 +17,43 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float gate_value(float g, int act) {
-  switch (act) {
-    case HEXLIB_B200_GATE_SIGMOID: return __fdividef(1.f, 1.f + expf(-g));
-    case HEXLIB_B200_GATE_SILU: return __fdividef(g, 1.f + expf(-g));
-    case HEXLIB_B200_GATE_TANH: return tanhf(g);
-  }
-  return g;
+// 1 / (1 + e^-g) of a pair of fp16 values. e^-g = 2^(-g L), L = log2(e): with L cut
+// to its first 13 bits the product by g's 11 is exact, and what was cut enters as
+// 1 + d, d = -g (L - L13) ln 2 (|d| < 2^-9 where the result is above 2^-32), so the
+// error is that of 2^x and the reciprocal, a few 2^-23.
+__device__ __forceinline__ float2 sigmoid2(float2 g) {
+  constexpr float L13 = 1.442626953125f;
+  constexpr float D = 4.719484e-5f;                   // (log2(e) - L13) ln 2
+  const float2 t = __fmul2_rn(g, make_float2(-L13, -L13));
+  float2 e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  float2 d = __fmul2_rn(g, make_float2(-D, -D));
+  d = make_float2(fmaxf(d.x, -1.f), fmaxf(d.y, -1.f));   // an infinite g: 0 (1 + d) is 0
+  e = __fadd2_rn(__ffma2_rn(e, d, e), make_float2(1.f, 1.f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+  return r;
 }
 
-// The gate's function of a pair, its branch taken once for eight values.
+// The gate's function of eight values, its branch taken once.
 __device__ __forceinline__ void gate_values(float2 (&g)[4], int act) {
-  if (act == HEXLIB_B200_GATE_NONE) return;
+  if (act == HEXLIB_B200_GATE_SIGMOID) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) g[q] = make_float2(gate_value(g[q].x, act), gate_value(g[q].y, act));
+    for (int q = 0; q < 4; ++q) g[q] = sigmoid2(g[q]);
+  } else if (act == HEXLIB_B200_GATE_SILU) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) g[q] = __fmul2_rn(g[q], sigmoid2(g[q]));
+  } else if (act == HEXLIB_B200_GATE_TANH) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) g[q] = make_float2(tanhf(g[q].x), tanhf(g[q].y));
+  }
+}
+__device__ __forceinline__ float gate_value(float g, int act) {
+  if (act == HEXLIB_B200_GATE_NONE) return g;
+  if (act == HEXLIB_B200_GATE_TANH) return tanhf(g);
+  const float s = sigmoid2(make_float2(g, g)).x;
+  return act == HEXLIB_B200_GATE_SILU ? g * s : s;
 }
 
 // A pair of a norm's values, every rounding written out (two-wide instructions round
@@ -320,6 +344,11 @@ int with_layout(int C, F&& f) {
   return f(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
 }
 
+// CTAs of a form that are resident on the device at once, found when it is loaded (a
+// grid of more would leave a partial last wave: 1184 CTAs on 444 measured 11 % slower).
+template <int G, int V, int VEC, bool E4M3>
+std::atomic<int> g_resident{0};
+
 template <int VEC, bool E4M3>
 int launch_form(const EdgeDesc& d, cudaStream_t s) {
   return with_layout(d.C, [&](auto G, auto V) {
@@ -328,8 +357,9 @@ int launch_form(const EdgeDesc& d, cudaStream_t s) {
     } else {
       const int64_t rows = G.value == 32 ? kThreads / 32 : 1;
       const int64_t ctas = (d.R + rows - 1) / rows;
+      const int64_t most = g_resident<G.value, V.value, VEC, E4M3>.load(std::memory_order_relaxed);
       edge_held<G.value, V.value, VEC, E4M3>
-          <<<(unsigned)(ctas < 148 * 8 ? ctas : 148 * 8), kThreads, 0, s>>>(d);
+          <<<(unsigned)(ctas < most ? ctas : most), kThreads, 0, s>>>(d);
     }
     if (cudaPeekAtLastError() != cudaSuccess) {
       cudaGetLastError();
@@ -340,14 +370,18 @@ int launch_form(const EdgeDesc& d, cudaStream_t s) {
 }
 
 template <int VEC, bool E4M3>
-bool load_form() {
+bool load_form(int sms) {
   cudaFuncAttributes a;
   bool ok = cudaFuncGetAttributes(&a, (const void*)edge_wide<E4M3>) == cudaSuccess;
   for (int C : {256, 512, 768, 1024, 2048, 4096, 6144, 8192, 16384})
     with_layout(C, [&](auto G, auto V) {
-      if constexpr (G.value != 0)
-        ok = ok && cudaFuncGetAttributes(
-                       &a, (const void*)edge_held<G.value, V.value, VEC, E4M3>) == cudaSuccess;
+      if constexpr (G.value != 0) {
+        int n = 0;
+        ok = ok && cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+                       &n, (const void*)edge_held<G.value, V.value, VEC, E4M3>, kThreads, 0) ==
+                       cudaSuccess && n > 0;
+        g_resident<G.value, V.value, VEC, E4M3>.store(n * sms, std::memory_order_relaxed);
+      }
       return 0;
     });
   return ok;
@@ -357,8 +391,11 @@ bool load_form() {
 
 // Load the kernels now, so that none is loaded lazily inside a graph capture.
 int edge_kernels_init() {
-  if (!load_form<8, false>() || !load_form<8, true>() || !load_form<1, false>() ||
-      !load_form<1, true>()) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      !load_form<8, false>(sms) || !load_form<8, true>(sms) || !load_form<1, false>(sms) ||
+      !load_form<1, true>(sms)) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }

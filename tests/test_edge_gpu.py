@@ -192,3 +192,21 @@ def test_the_separate_quantization_agrees_on_the_device():
     _, (q, s) = run(c, 1, e4m3=True)
     q2, s2 = quantize(h)
     assert np.array_equal(U.host(q), U.host(q2)) and np.array_equal(U.host(s), U.host(s2))
+
+
+@pytest.mark.parametrize("act", [1, 2, 3])
+@pytest.mark.parametrize("C", [1024, 1203, 17000])
+def test_gates_of_every_size(C, act):
+    # gates over fp16's whole range on a branch of ones: x' is the gate's function
+    rng = np.random.default_rng(act)
+    g = (rng.standard_normal((8, C)) * 2.0 ** rng.integers(-12, 5, (8, C))).astype(np.float16)
+    g[0, :8] = [0, -0.0, 65504, -65504, 17, -17, 6e-8, -11]
+    one = np.ones((8, C), np.float16)
+    c = dict(x=one, y=one, post_w=None, post_b=None, gate=g, pre_w=None, pre_b=None)
+    xo, _ = run(c, act, xs=0.0)
+    ref, bound = B.edge_x(one, one, None, None, g, act, 0.0, 1.0, False, EPS)
+    B.assert_within(U.host(xo), ref, bound, "gate")
+    g[0, :2] = [np.inf, -np.inf]
+    got = U.host(run(c, act, xs=0.0)[0])[0, :2]
+    want = {1: [1, 0], 2: [np.inf, np.nan], 3: [1, -1]}[act]
+    assert np.array_equal(got.astype(np.float64), np.array(want, np.float64), equal_nan=True)
