@@ -58,26 +58,24 @@ __device__ __forceinline__ float gate_value(float g, int act) {
 
 // A pair of a norm's values, every rounding written out (two-wide instructions round
 // both as the scalar ones do): every form gives the same bits from the same moments.
-// `shift` is minus the mean.
-__device__ __forceinline__ float2 normed2(float2 v, float shift, float inv, float2 w, bool has_b,
-                                          float2 b) {
+// `shift` is minus the mean; b is 0 where there is none.
+__device__ __forceinline__ float2 normed2(float2 v, float shift, float inv, float2 w, float2 b) {
   v = __fmul2_rn(__fadd2_rn(v, make_float2(shift, shift)), make_float2(inv, inv));
-  return has_b ? __ffma2_rn(v, w, b) : __fmul2_rn(v, w);
+  return __ffma2_rn(v, w, b);
 }
-__device__ __forceinline__ float normed(float v, float2 ms, float w, bool has_b, float b) {
-  v = __fmul_rn(__fsub_rn(v, ms.x), ms.y);
-  return has_b ? fmaf(v, w, b) : __fmul_rn(v, w);
+__device__ __forceinline__ float normed(float v, float2 ms, float w, float b) {
+  return fmaf(__fmul_rn(__fsub_rn(v, ms.x), ms.y), w, b);
 }
 __device__ __forceinline__ float blended(float x_scale, float x, float y_scale, float u) {
   return fmaf(x_scale, x, __fmul_rn(y_scale, u));
 }
 
-// Sum over the G threads of a row: a warp, or the CTA through shared memory. The
-// slots rotate, so that one barrier a sum suffices: a slot is written again only
-// three barriers after it was read.
+// Sum over the G threads of a row: a warp, or the CTA of G threads through shared
+// memory. The slots rotate, so that one barrier a sum suffices: a slot is written
+// again only three barriers after it was read.
 template <int G>
 struct RowSum {
-  float (*red)[kThreads / 32];
+  float (*red)[8];
   int slot = 0;
   __device__ float operator()(float v) {
 #pragma unroll
@@ -87,10 +85,13 @@ struct RowSum {
     slot = (slot + 1) & 3;
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < G / 32; ++i) t += r[i];
-    return t;
+    const float4 a = *reinterpret_cast<const float4*>(r);
+    v = (a.x + a.y) + (a.z + a.w);
+    if constexpr (G == 256) {
+      const float4 b = *reinterpret_cast<const float4*>(r + 4);
+      v += (b.x + b.y) + (b.z + b.w);
+    }
+    return v;
   }
 };
 
@@ -117,18 +118,19 @@ __device__ __forceinline__ void load8f(float2 (&f)[4], const float* p, int left)
                          2 * q + 1 < left ? __ldg(p + 2 * q + 1) : 0.f);
   }
 }
-// Zeros from `left` on (a multiple of 8 when VEC is 8, so the whole vector or nothing).
+// A pair with zeros from `left` on. With VEC 8 a vector is in the row or not, which the
+// callers know.
 template <int VEC>
 __device__ __forceinline__ uint32_t pack_in(float2 f, int q, int left) {
-  if constexpr (VEC == 8) return left > 0 ? pack(f.x, f.y) : 0u;
+  if constexpr (VEC == 8) return pack(f.x, f.y);
   return pack(2 * q < left ? f.x : 0.f, 2 * q + 1 < left ? f.y : 0.f);
 }
 
 // mean (0 for rms) and 1 / sqrt(mean squared deviation + eps) of a row of C values in
 // registers: vector j of thread g at column (j G + g) 8, zeros past C.
 template <int G, int V, int VEC>
-__device__ __forceinline__ float2 moments(const uint32_t (&w)[V][4], int g, int C, bool layer,
-                                          float eps, RowSum<G>& sum) {
+__device__ __forceinline__ float2 moments(const uint32_t (&w)[V][4], int g, int C, float per_c,
+                                          bool layer, float eps, RowSum<G>& sum) {
   float mean = 0.f;
   if (layer) {
     float2 s = make_float2(0.f, 0.f);
@@ -136,7 +138,7 @@ __device__ __forceinline__ float2 moments(const uint32_t (&w)[V][4], int g, int 
     for (int j = 0; j < V; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) s = __fadd2_rn(s, halves(w[j][q]));
-    mean = sum(s.x + s.y) / C;
+    mean = sum(s.x + s.y) * per_c;
   }
   const float2 shift = make_float2(-mean, -mean);
   float2 ss = make_float2(0.f, 0.f);
@@ -152,59 +154,58 @@ __device__ __forceinline__ float2 moments(const uint32_t (&w)[V][4], int g, int 
       ss = __ffma2_rn(f, f, ss);
     }
   }
-  return make_float2(mean, 1.f / sqrtf(sum(ss.x + ss.y) / C + eps));
+  return make_float2(mean, rsqrtf(fmaf(sum(ss.x + ss.y), per_c, eps)));
 }
 
 // A row of up to G * V * 8 values in the registers of G threads (a warp, or the CTA),
 // read once and written once; its gate is read with it, ahead of the sums.
+constexpr int held_threads(int G) { return G == 32 ? 256 : G; }
+constexpr int held_ctas(int G, int V) {       // of an SM: registers for V vectors of x, y, gate
+  return (V == 1 ? 1024 : V <= 3 ? 768 : V == 4 ? 512 : 256) / held_threads(G);
+}
 template <int G, int V, int VEC, bool E4M3>
-__global__ void __launch_bounds__(kThreads, V == 1 ? 4 : V <= 3 ? 3 : V == 4 ? 2 : 1)
-    edge_held(const EdgeDesc d) {
-  __shared__ float red[4][kThreads / 32];
+__global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(const EdgeDesc d) {
+  __shared__ __align__(16) float red[4][8];
   RowSum<G> sum{red};
+  constexpr int ROWS = G == 32 ? held_threads(G) / 32 : 1;
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
   const int g = G == 32 ? (threadIdx.x & 31) : threadIdx.x;
   const int per_gate = d.gate ? d.R / d.gate_rows : 1;
   const int C = d.C, blocks = (C + 127) / 128, padded = (blocks + 3) / 4 * 4;
-  const int64_t first = G == 32 ? blockIdx.x * (int64_t)(kThreads / 32) + (threadIdx.x >> 5)
-                                : (int64_t)blockIdx.x;
-  const int64_t step = G == 32 ? (int64_t)gridDim.x * (kThreads / 32) : (int64_t)gridDim.x;
-  for (int64_t r = first; r < d.R; r += step) {
+  const float per_c = 1.f / C;
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  for (int64_t r = blockIdx.x * (int64_t)ROWS + (G == 32 ? threadIdx.x >> 5 : 0); r < d.R;
+       r += step) {
+    const int64_t at = r * C + g * 8;             // of vector 0; vector j is G * 8 further
     uint32_t x[V][4];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (j * G + g) * 8;
-      load8<VEC>(x[j], (const __half*)d.x + r * C + c, C - c);
-    }
+    for (int j = 0; j < V; ++j)
+      load8<VEC>(x[j], (const __half*)d.x + at + j * G * 8, C - (j * G + g) * 8);
     if (d.y) {
       uint32_t y[V][4], gate[V][4];
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = (j * G + g) * 8;
-        load8<VEC>(y[j], (const __half*)d.y + r * C + c, C - c);
-      }
+      for (int j = 0; j < V; ++j)
+        load8<VEC>(y[j], (const __half*)d.y + at + j * G * 8, C - (j * G + g) * 8);
       if (d.gate) {
+        const __half* gp = (const __half*)d.gate + (int64_t)((int)r / per_gate) * C + g * 8;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = (j * G + g) * 8;
-          load8<VEC>(gate[j], (const __half*)d.gate + (r / per_gate) * C + c, C - c);
-        }
+        for (int j = 0; j < V; ++j) load8<VEC>(gate[j], gp + j * G * 8, C - (j * G + g) * 8);
       }
       float2 ms = make_float2(0.f, 1.f);
-      if (d.post_w) ms = moments<G, V, VEC>(y, g, C, layer, d.eps, sum);
+      if (d.post_w) ms = moments<G, V, VEC>(y, g, C, per_c, layer, d.eps, sum);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const int c = (j * G + g) * 8;
+        if (VEC == 8 && c >= C) continue;
         float2 u[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) u[q] = halves(y[j][q]);
         if (d.post_w) {
-          float2 w[4], b[4];
+          float2 w[4], b[4] = {};
           load8f<VEC>(w, d.post_w + c, C - c);
           if (d.post_b) load8f<VEC>(b, d.post_b + c, C - c);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            u[q] = normed2(u[q], -ms.x, ms.y, w[q], d.post_b != nullptr, b[q]);
+          for (int q = 0; q < 4; ++q) u[q] = normed2(u[q], -ms.x, ms.y, w[q], b[q]);
         }
         if (d.gate) {
           float2 f[4];
@@ -218,27 +219,29 @@ __global__ void __launch_bounds__(kThreads, V == 1 ? 4 : V <= 3 ? 3 : V == 4 ? 2
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           x[j][q] = pack_in<VEC>(__ffma2_rn(xs, halves(x[j][q]), __fmul2_rn(ys, u[q])), q, C - c);
-        store8<VEC>((__half*)d.x_out + r * C + c, x[j], C - c);
+        store8<VEC>((__half*)d.x_out + at + j * G * 8, x[j], C - c);
       }
     }
     if (!d.pre_w) continue;
-    const float2 ms = moments<G, V, VEC>(x, g, C, layer, d.eps, sum);
+    const float2 ms = moments<G, V, VEC>(x, g, C, per_c, layer, d.eps, sum);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (j * G + g) * 8;
-      float2 w[4], b[4];
-      load8f<VEC>(w, d.pre_w + c, C - c);
-      if (d.pre_b) load8f<VEC>(b, d.pre_b + c, C - c);
-      uint32_t h[4];
+      uint32_t h[4] = {0, 0, 0, 0};
+      if (VEC != 8 || c < C) {
+        float2 w[4], b[4] = {};
+        load8f<VEC>(w, d.pre_w + c, C - c);
+        if (d.pre_b) load8f<VEC>(b, d.pre_b + c, C - c);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        h[q] = pack_in<VEC>(normed2(halves(x[j][q]), -ms.x, ms.y, w[q], d.pre_b != nullptr, b[q]),
-                            q, C - c);
+        for (int q = 0; q < 4; ++q)
+          h[q] = pack_in<VEC>(normed2(halves(x[j][q]), -ms.x, ms.y, w[q], b[q]), q, C - c);
+      }
       if constexpr (!E4M3) {
-        store8<VEC>((__half*)d.h + r * C + c, h, C - c);
+        store8<VEC>((__half*)d.h + at + j * G * 8, h, C - c);
       } else {
         // 16 consecutive threads hold a block; blocks past the last are zeros
         const int b128 = c >> 7;
+        __syncwarp();
         uint32_t byte;
         const uint2 codes = e4m3_encode8(h, 0xffffu << (threadIdx.x & 16), byte);
         if (b128 < blocks)
@@ -257,28 +260,29 @@ __global__ void __launch_bounds__(kThreads, V == 1 ? 4 : V <= 3 ? 3 : V == 4 ? 2
 
 // Rows wider than the registers hold: one CTA per row, read again for each pass. A
 // thread reads x' of other threads' columns only after the barriers of the sums.
-__device__ __forceinline__ float2 moments_wide(const __half* v, int C, bool layer, float eps,
-                                               RowSum<kThreads>& sum) {
+__device__ __forceinline__ float2 moments_wide(const __half* v, int C, float per_c, bool layer,
+                                               float eps, RowSum<kThreads>& sum) {
   float mean = 0.f;
   if (layer) {
     float s = 0.f;
     for (int c = threadIdx.x; c < C; c += kThreads) s += __half2float(v[c]);
-    mean = sum(s) / C;
+    mean = sum(s) * per_c;
   }
   float ss = 0.f;
   for (int c = threadIdx.x; c < C; c += kThreads) {
     const float d = __half2float(v[c]) - mean;
     ss = fmaf(d, d, ss);
   }
-  return make_float2(mean, 1.f / sqrtf(sum(ss) / C + eps));
+  return make_float2(mean, rsqrtf(fmaf(sum(ss), per_c, eps)));
 }
 
 template <bool E4M3>
 __global__ void __launch_bounds__(kThreads) edge_wide(const EdgeDesc d) {
-  __shared__ float red[4][kThreads / 32];
+  __shared__ __align__(16) float red[4][8];
   RowSum<kThreads> sum{red};
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
   const int per_gate = d.gate ? d.R / d.gate_rows : 1;
+  const float per_c = 1.f / d.C;
   for (int64_t r = blockIdx.x; r < d.R; r += gridDim.x) {
     const __half* x = (const __half*)d.x + r * d.C;
     if (d.y) {
@@ -286,19 +290,19 @@ __global__ void __launch_bounds__(kThreads) edge_wide(const EdgeDesc d) {
       const __half* gate = (const __half*)d.gate + (r / per_gate) * d.C;
       __half* xo = (__half*)d.x_out + r * d.C;
       float2 ms = make_float2(0.f, 1.f);
-      if (d.post_w) ms = moments_wide(y, d.C, layer, d.eps, sum);
+      if (d.post_w) ms = moments_wide(y, d.C, per_c, layer, d.eps, sum);
       for (int c = threadIdx.x; c < d.C; c += kThreads) {
         float u = __half2float(y[c]);
-        if (d.post_w) u = normed(u, ms, d.post_w[c], d.post_b, d.post_b ? d.post_b[c] : 0.f);
+        if (d.post_w) u = normed(u, ms, d.post_w[c], d.post_b ? d.post_b[c] : 0.f);
         if (d.gate) u = __fmul_rn(u, gate_value(__half2float(gate[c]), d.gate_act));
         xo[c] = __float2half_rn(blended(d.x_scale, __half2float(x[c]), d.y_scale, u));
       }
       x = xo;
     }
     if (!d.pre_w) continue;
-    const float2 ms = moments_wide(x, d.C, layer, d.eps, sum);
+    const float2 ms = moments_wide(x, d.C, per_c, layer, d.eps, sum);
     auto h_of = [&](int c) {
-      return __float2half_rn(normed(__half2float(x[c]), ms, d.pre_w[c], d.pre_b,
+      return __float2half_rn(normed(__half2float(x[c]), ms, d.pre_w[c],
                                     d.pre_b ? d.pre_b[c] : 0.f));
     };
     if constexpr (!E4M3) {
@@ -335,8 +339,9 @@ int with_layout(int C, F&& f) {
   HB_EDGE_LAYOUT(32, 2)
   HB_EDGE_LAYOUT(32, 3)
   HB_EDGE_LAYOUT(32, 4)
-  HB_EDGE_LAYOUT(256, 1)
-  HB_EDGE_LAYOUT(256, 2)
+  HB_EDGE_LAYOUT(128, 2)
+  HB_EDGE_LAYOUT(128, 3)
+  HB_EDGE_LAYOUT(128, 4)
   HB_EDGE_LAYOUT(256, 3)
   HB_EDGE_LAYOUT(256, 4)
   HB_EDGE_LAYOUT(256, 8)
@@ -355,11 +360,11 @@ int launch_form(const EdgeDesc& d, cudaStream_t s) {
     if constexpr (G.value == 0) {
       edge_wide<E4M3><<<d.R < 148 * 8 ? d.R : 148 * 8, kThreads, 0, s>>>(d);
     } else {
-      const int64_t rows = G.value == 32 ? kThreads / 32 : 1;
+      const int64_t rows = G.value == 32 ? held_threads(32) / 32 : 1;
       const int64_t ctas = (d.R + rows - 1) / rows;
       const int64_t most = g_resident<G.value, V.value, VEC, E4M3>.load(std::memory_order_relaxed);
       edge_held<G.value, V.value, VEC, E4M3>
-          <<<(unsigned)(ctas < most ? ctas : most), kThreads, 0, s>>>(d);
+          <<<(unsigned)(ctas < most ? ctas : most), held_threads(G.value), 0, s>>>(d);
     }
     if (cudaPeekAtLastError() != cudaSuccess) {
       cudaGetLastError();
@@ -373,13 +378,13 @@ template <int VEC, bool E4M3>
 bool load_form(int sms) {
   cudaFuncAttributes a;
   bool ok = cudaFuncGetAttributes(&a, (const void*)edge_wide<E4M3>) == cudaSuccess;
-  for (int C : {256, 512, 768, 1024, 2048, 4096, 6144, 8192, 16384})
+  for (int C : {256, 512, 768, 1024, 2048, 3000, 4096, 6144, 8192, 16384})
     with_layout(C, [&](auto G, auto V) {
       if constexpr (G.value != 0) {
         int n = 0;
         ok = ok && cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-                       &n, (const void*)edge_held<G.value, V.value, VEC, E4M3>, kThreads, 0) ==
-                       cudaSuccess && n > 0;
+                       &n, (const void*)edge_held<G.value, V.value, VEC, E4M3>,
+                       held_threads(G.value), 0) == cudaSuccess && n > 0;
         g_resident<G.value, V.value, VEC, E4M3>.store(n * sms, std::memory_order_relaxed);
       }
       return 0;
