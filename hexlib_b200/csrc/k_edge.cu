@@ -36,19 +36,6 @@ __device__ __forceinline__ float2 sigmoid2(float2 g) {
   return r;
 }
 
-// The gate's function of eight values, its branch taken once.
-__device__ __forceinline__ void gate_values(float2 (&g)[4], int act) {
-  if (act == HEXLIB_B200_GATE_SIGMOID) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) g[q] = sigmoid2(g[q]);
-  } else if (act == HEXLIB_B200_GATE_SILU) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) g[q] = __fmul2_rn(g[q], sigmoid2(g[q]));
-  } else if (act == HEXLIB_B200_GATE_TANH) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) g[q] = make_float2(tanhf(g[q].x), tanhf(g[q].y));
-  }
-}
 __device__ __forceinline__ float gate_value(float g, int act) {
   if (act == HEXLIB_B200_GATE_NONE) return g;
   if (act == HEXLIB_B200_GATE_TANH) return tanhf(g);
@@ -56,13 +43,6 @@ __device__ __forceinline__ float gate_value(float g, int act) {
   return act == HEXLIB_B200_GATE_SILU ? g * s : s;
 }
 
-// A pair of a norm's values, every rounding written out (two-wide instructions round
-// both as the scalar ones do): every form gives the same bits from the same moments.
-// `shift` is minus the mean; b is 0 where there is none.
-__device__ __forceinline__ float2 normed2(float2 v, float shift, float inv, float2 w, float2 b) {
-  v = __fmul2_rn(__fadd2_rn(v, make_float2(shift, shift)), make_float2(inv, inv));
-  return __ffma2_rn(v, w, b);
-}
 __device__ __forceinline__ float normed(float v, float2 ms, float w, float b) {
   return fmaf(__fmul_rn(__fsub_rn(v, ms.x), ms.y), w, b);
 }
@@ -126,42 +106,99 @@ __device__ __forceinline__ uint32_t pack_in(float2 f, int q, int left) {
   return pack(2 * q < left ? f.x : 0.f, 2 * q + 1 < left ? f.y : 0.f);
 }
 
-// mean (0 for rms) and 1 / sqrt(mean squared deviation + eps) of a row of C values in
-// registers: vector j of thread g at column (j G + g) 8, zeros past C.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// A row in the registers of the G threads that share it, as floats: vector j of thread
+// g is columns (j G + g) 8 and on, zeros past C. Each step runs over all V vectors
+// between two branches, so that their chains overlap, in two-wide instructions with
+// every rounding written out: the fp16 and the 8-bit form give the same bits.
 template <int G, int V, int VEC>
-__device__ __forceinline__ float2 moments(const uint32_t (&w)[V][4], int g, int C, float per_c,
-                                          bool layer, float eps, RowSum<G>& sum) {
-  float mean = 0.f;
-  if (layer) {
-    float2 s = make_float2(0.f, 0.f);
+struct Row {
+  float2 v[V][4];
+
+  __device__ __forceinline__ void unpack(const uint32_t (&w)[V][4]) {
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) s = __fadd2_rn(s, halves(w[j][q]));
-    mean = sum(s.x + s.y) * per_c;
+      for (int q = 0; q < 4; ++q) v[j][q] = halves(w[j][q]);
   }
-  const float2 shift = make_float2(-mean, -mean);
-  float2 ss = make_float2(0.f, 0.f);
+
+  // norm(v) w + b, the moments taken over the whole row (the squared deviations of a
+  // layer norm after its mean). v inv - mean inv is one fused step a pair.
+  __device__ __forceinline__ void norm(const float* w, const float* b, int g, int C, float per_c,
+                                       bool layer, float eps, RowSum<G>& sum) {
+    float2 ss = both(0.f);
+    float mean = 0.f;
+    if (layer) {
+      float2 s = both(0.f);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int left = C - (j * G + g) * 8;
-    if (VEC == 8 && left <= 0) continue;
+      for (int j = 0; j < V; ++j)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float2 f = __fadd2_rn(halves(w[j][q]), shift);
-      if (VEC != 8 && 2 * q >= left) f.x = 0.f;
-      if (VEC != 8 && 2 * q + 1 >= left) f.y = 0.f;
-      ss = __ffma2_rn(f, f, ss);
+        for (int q = 0; q < 4; ++q) s = __fadd2_rn(s, v[j][q]);
+      mean = sum(s.x + s.y) * per_c;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int left = C - (j * G + g) * 8;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float2 d = __fadd2_rn(v[j][q], both(-mean));
+          if ((VEC == 8 ? 0 : 2 * q) >= left) d.x = 0.f;
+          if ((VEC == 8 ? 0 : 2 * q + 1) >= left) d.y = 0.f;
+          ss = __ffma2_rn(d, d, ss);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ss = __ffma2_rn(v[j][q], v[j][q], ss);
+    }
+    const float inv = rsqrtf(fmaf(sum(ss.x + ss.y), per_c, eps));
+    const float2 shift = both(-__fmul_rn(mean, inv));
+    if (b) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = (j * G + g) * 8;
+        float2 wv[4], bv[4];
+        load8f<VEC>(wv, w + c, C - c);
+        load8f<VEC>(bv, b + c, C - c);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          v[j][q] = __ffma2_rn(__ffma2_rn(v[j][q], both(inv), shift), wv[q], bv[q]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = (j * G + g) * 8;
+        float2 wv[4];
+        load8f<VEC>(wv, w + c, C - c);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          v[j][q] = __fmul2_rn(__ffma2_rn(v[j][q], both(inv), shift), wv[q]);
+      }
     }
   }
-  return make_float2(mean, rsqrtf(fmaf(sum(ss.x + ss.y), per_c, eps)));
-}
+
+  // v *= f(gate)
+  __device__ __forceinline__ void gated(const uint32_t (&gate)[V][4], int act) {
+    auto times = [&](auto f) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[j][q] = __fmul2_rn(v[j][q], f(halves(gate[j][q])));
+    };
+    if (act == HEXLIB_B200_GATE_NONE) times([](float2 x) { return x; });
+    else if (act == HEXLIB_B200_GATE_SIGMOID) times([](float2 x) { return sigmoid2(x); });
+    else if (act == HEXLIB_B200_GATE_SILU) times([](float2 x) { return __fmul2_rn(x, sigmoid2(x)); });
+    else times([](float2 x) { return make_float2(tanhf(x.x), tanhf(x.y)); });
+  }
+};
 
 // A row of up to G * V * 8 values in the registers of G threads (a warp, or the CTA),
 // read once and written once; its gate is read with it, ahead of the sums.
-constexpr int held_threads(int G) { return G == 32 ? 256 : G; }
+constexpr int held_threads(int G) { return G == 32 ? 128 : G; }
 constexpr int held_ctas(int G, int V) {       // of an SM: registers for V vectors of x, y, gate
-  return (V == 1 ? 1024 : V <= 3 ? 768 : V == 4 ? 512 : 256) / held_threads(G);
+  return (V == 1 ? 1024 : V == 2 ? 768 : V == 3 ? 640 : V == 4 ? 512 : 256) / held_threads(G);
 }
 template <int G, int V, int VEC, bool E4M3>
 __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(const EdgeDesc d) {
@@ -181,6 +218,7 @@ __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(co
 #pragma unroll
     for (int j = 0; j < V; ++j)
       load8<VEC>(x[j], (const __half*)d.x + at + j * G * 8, C - (j * G + g) * 8);
+    Row<G, V, VEC> v;
     if (d.y) {
       uint32_t y[V][4], gate[V][4];
 #pragma unroll
@@ -191,57 +229,35 @@ __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(co
 #pragma unroll
         for (int j = 0; j < V; ++j) load8<VEC>(gate[j], gp + j * G * 8, C - (j * G + g) * 8);
       }
-      float2 ms = make_float2(0.f, 1.f);
-      if (d.post_w) ms = moments<G, V, VEC>(y, g, C, per_c, layer, d.eps, sum);
+      v.unpack(y);
+      if (d.post_w) v.norm(d.post_w, d.post_b, g, C, per_c, layer, d.eps, sum);
+      if (d.gate) v.gated(gate, d.gate_act);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int c = (j * G + g) * 8;
-        if (VEC == 8 && c >= C) continue;
-        float2 u[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) u[q] = halves(y[j][q]);
-        if (d.post_w) {
-          float2 w[4], b[4] = {};
-          load8f<VEC>(w, d.post_w + c, C - c);
-          if (d.post_b) load8f<VEC>(b, d.post_b + c, C - c);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) u[q] = normed2(u[q], -ms.x, ms.y, w[q], b[q]);
-        }
-        if (d.gate) {
-          float2 f[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) f[q] = halves(gate[j][q]);
-          gate_values(f, d.gate_act);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) u[q] = __fmul2_rn(u[q], f[q]);
-        }
-        const float2 xs = make_float2(d.x_scale, d.x_scale), ys = make_float2(d.y_scale, d.y_scale);
+        const int left = C - (j * G + g) * 8;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          x[j][q] = pack_in<VEC>(__ffma2_rn(xs, halves(x[j][q]), __fmul2_rn(ys, u[q])), q, C - c);
-        store8<VEC>((__half*)d.x_out + at + j * G * 8, x[j], C - c);
+          x[j][q] = pack_in<VEC>(__ffma2_rn(both(d.x_scale), halves(x[j][q]),
+                                            __fmul2_rn(both(d.y_scale), v.v[j][q])), q, left);
+        store8<VEC>((__half*)d.x_out + at + j * G * 8, x[j], left);
+        if (VEC == 8 && left <= 0) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0;
       }
     }
     if (!d.pre_w) continue;
-    const float2 ms = moments<G, V, VEC>(x, g, C, per_c, layer, d.eps, sum);
+    v.unpack(x);
+    v.norm(d.pre_w, d.pre_b, g, C, per_c, layer, d.eps, sum);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (j * G + g) * 8;
-      uint32_t h[4] = {0, 0, 0, 0};
-      if (VEC != 8 || c < C) {
-        float2 w[4], b[4] = {};
-        load8f<VEC>(w, d.pre_w + c, C - c);
-        if (d.pre_b) load8f<VEC>(b, d.pre_b + c, C - c);
+      uint32_t h[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          h[q] = pack_in<VEC>(normed2(halves(x[j][q]), -ms.x, ms.y, w[q], b[q]), q, C - c);
-      }
+      for (int q = 0; q < 4; ++q) h[q] = pack_in<VEC>(v.v[j][q], q, C - c);
       if constexpr (!E4M3) {
         store8<VEC>((__half*)d.h + at + j * G * 8, h, C - c);
       } else {
         // 16 consecutive threads hold a block; blocks past the last are zeros
         const int b128 = c >> 7;
-        __syncwarp();
+        if (VEC == 8 && c >= C) h[0] = h[1] = h[2] = h[3] = 0;
         uint32_t byte;
         const uint2 codes = e4m3_encode8(h, 0xffffu << (threadIdx.x & 16), byte);
         if (b128 < blocks)
