@@ -222,6 +222,15 @@ __device__ __forceinline__ void tma_load_3d_pair(const CUtensorMap* map, uint32_
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_t bar_caddr,
+                                                 void* smem_dst, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::"
+      "bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(map), "r"(bar_caddr), "r"(c0), "r"(c1)
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -352,6 +361,26 @@ __device__ __forceinline__ void umma_e4m3_scaled(uint32_t d_tmem, uint64_t adesc
       "[%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accum)
       : "memory");
+}
+
+// The pair form: M = 256 rows, 128 from each CTA, N columns, N / 2 from each CTA's B
+// tile; each CTA's tensor memory holds the scales of its own rows of A and of all N.
+__device__ __forceinline__ void umma_e4m3_scaled_pair(uint32_t d_tmem, uint64_t adesc,
+                                                      uint64_t bdesc, uint32_t idesc,
+                                                      uint32_t sfa, uint32_t sfb,
+                                                      uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X "
+      "[%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accum)
+      : "memory");
+}
+// In both CTAs of the pair, from each one's shared memory to its tensor memory.
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint64_t sdesc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(sdesc)
+               : "memory");
 }
 
 // Copy 32 rows of 16 bytes from shared memory to four columns of tensor memory,

@@ -13,6 +13,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "hb_device.cuh"
 #include "hb_e4m3.cuh"
 #include "hb_kernels.h"
@@ -240,6 +242,29 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
+E4m3Params params_of(const GemmE4m3Desc& g, int* err) {
+  E4m3Params p = {};
+  p.a_scales = g.a_scales;
+  p.w_scales = g.w_scales;
+  p.bias = g.bias;
+  p.resid = (const __half*)g.resid;
+  p.out = (__half*)g.out;
+  p.M = g.M;
+  p.N = g.N;
+  p.num_kb = (int)(e4m3_pitch(g.K) / kBlockK);
+  p.act = g.act;
+  p.err = err;
+  return p;
+}
+
+cudaLaunchAttribute* cluster_of(cudaLaunchAttribute* attr, int n) {
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)n;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  return attr;
+}
+
 template <int BN>
 int launch_tile(const GemmE4m3Desc& g, int split, int* err, cudaStream_t s) {
   using Cfg = TileCfg<BN>;
@@ -248,18 +273,8 @@ int launch_tile(const GemmE4m3Desc& g, int split, int* err, cudaStream_t s) {
   if (!make_tmap_2d_u8(&tw, g.w, pitch, (uint64_t)g.N, 128) ||
       !make_tmap_2d_u8(&ta, g.a, pitch, (uint64_t)g.M, BN))
     return HEXLIB_B200_ERR_CUDA;
-  E4m3Params p;
-  p.a_scales = g.a_scales;
-  p.w_scales = g.w_scales;
-  p.bias = g.bias;
-  p.resid = (const __half*)g.resid;
-  p.out = (__half*)g.out;
-  p.M = g.M;
-  p.N = g.N;
-  p.num_kb = (int)(pitch / kBlockK);
-  p.act = g.act;
+  E4m3Params p = params_of(g, err);
   p.tiles_n = (g.N + 127) / 128;
-  p.err = err;
   const int64_t tiles = (int64_t)p.tiles_n * ((g.M + BN - 1) / BN);
   if (tiles * split > 0x7fffffff) return HEXLIB_B200_ERR_INVAL_PARAMS;
   cudaLaunchConfig_t cfg = {};
@@ -268,17 +283,352 @@ int launch_tile(const GemmE4m3Desc& g, int split, int* err, cudaStream_t s) {
   cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)split;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
+  cfg.attrs = cluster_of(attr, split);
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, gemm_e4m3_tile<BN>, tw, ta, p, split) != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
   return HEXLIB_B200_OK;
+}
+
+// ---- CTA pairs, 256 tokens by 256 features ---------------------------------------
+//
+// A persistent kernel on clusters of two SMs. Per block of 128 of K each CTA lands its
+// own 128 rows of a and of w (32 KiB), and the leader's MMA thread multiplies the
+// 256 x 256 x 128 block across both SMs: half the fill traffic of one-CTA tiles, which
+// is what bounds an 8-bit mainloop (64 bytes per cycle and SM even so).
+//
+// Tensor memory holds 512 columns: two 256-column accumulators would leave none for
+// the scales. The accumulators therefore OVERLAP by 24 columns, [0, 256) and
+// [232, 488), and the scales take [488, 512). The epilogue reads the overlap first and
+// tells the MMA thread as soon as it has; the next tile's MMAs start then, while the
+// rest of the tile is finished. That arrival also says that the warp is done with
+// every earlier tile, so one barrier covers both uses.
+//
+//   full[s]     leader: both CTAs' loads of stage s
+//   empty[s]    both: the stage has been read
+//   sf_full[b]  leader: both CTAs have written scale buffer b
+//   sf_empty[b] both: the MMAs that use scale buffer b are done
+//   tfull[a]    both: accumulator a is complete
+//   tempty      leader: the pair's 16 epilogue warps have read the overlap
+constexpr int kPairThreads = 352;   // loads, MMAs, scales, 8 epilogue warps
+
+struct PairCfg {
+  static constexpr int STAGES = 5;
+  static constexpr int HALF_BYTES = 128 * kBlockK;
+  static constexpr int STAGE_BYTES = 2 * HALF_BYTES;      // of each CTA
+  static constexpr int SF_BYTES = 512 + 1024;             // own rows of a, all rows of w
+  static constexpr int STAGING = 8 * 4096;                // a 32 x 64 fp16 box per warp
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING + 2 * SF_BYTES + 1024 + 256;
+  static constexpr uint32_t ACC1 = 232, SF = 488;
+};
+
+// 32 columns of a row: bias, activation, residual, one rounding.
+__device__ __forceinline__ void finish32(const E4m3Params& p, uint32_t (&v)[32], int64_t row,
+                                         int n, uint32_t (&w)[16]) {
+  const bool row_ok = row < p.M;
+  if (p.bias) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 b = n + j < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + n + j))
+                                   : make_float4(0, 0, 0, 0);
+      v[j] = __float_as_uint(__uint_as_float(v[j]) + b.x);
+      v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + b.y);
+      v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) + b.z);
+      v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) + b.w);
+    }
+  }
+  if (p.act == 1) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float2 g = gelu_tanh_f2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
+      v[j] = __float_as_uint(g.x);
+      v[j + 1] = __float_as_uint(g.y);
+    }
+  } else if (p.act == 2) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(gelu_erf_f(__uint_as_float(v[j])));
+  }
+  if (p.resid && row_ok) {
+    const __half* r = p.resid + row * p.N + n;
+#pragma unroll
+    for (int j = 0; j < 32; j += 8) {
+      const uint4 u = n + j < p.N ? *reinterpret_cast<const uint4*>(r + j) : make_uint4(0, 0, 0, 0);
+      const uint32_t h[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[q]));
+        v[j + 2 * q] = __float_as_uint(__uint_as_float(v[j + 2 * q]) + f.x);
+        v[j + 2 * q + 1] = __float_as_uint(__uint_as_float(v[j + 2 * q + 1]) + f.y);
+      }
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 16; ++q)
+    w[q] = pack_half2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1)
+    gemm_e4m3_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ CUtensorMap tmC, const E4m3Params p) {
+  using Cfg = PairCfg;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sW = smem + Cfg::STAGES * Cfg::HALF_BYTES;
+  uint8_t* sOut = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
+  uint8_t* sSF = sOut + Cfg::STAGING;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + 2 * Cfg::SF_BYTES);
+  uint64_t* empty = full + Cfg::STAGES;
+  uint64_t* sf_full = empty + Cfg::STAGES;
+  uint64_t* sf_empty = sf_full + 2;
+  uint64_t* tfull = sf_empty + 2;
+  uint64_t* tempty = tfull + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Cfg::STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&sf_full[b], 2);
+      mbar_init(&sf_empty[b], 1);
+      mbar_init(&tfull[b], 1);
+    }
+    mbar_init(tempty, 16);
+    *abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmC);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t peer_abort = cluster_addr(tmem_slot + 1, rank ^ 1u);
+
+  const int64_t total = (int64_t)((p.M + 255) / 256) * p.tiles_n;
+  const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t full_lead = cluster_addr(full, 0);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int64_t t = first; t < total; t += step) {
+        const int row = (int)(t / p.tiles_n) * 256 + (int)rank * 128;
+        const int col = (int)(t % p.tiles_n) * 256 + (int)rank * 128;
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          if (!mbar_wait_cluster(&empty[s], ph ^ 1u, abort_flag, p.err)) {
+            st_cluster_u32(peer_abort, 1);
+            goto out;
+          }
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE_BYTES);
+          tma_load_2d_pair(&tmA, full_lead + s * 8, sA + s * Cfg::HALF_BYTES, kb * kBlockK, row);
+          tma_load_2d_pair(&tmW, full_lead + s * 8, sW + s * Cfg::HALF_BYTES, kb * kBlockK, col);
+          if (++s == Cfg::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t idesc = idesc_e4m3_scaled(256, 256);
+      int s = 0, i = 0;
+      uint32_t ph = 0, u = 0;                        // u: scale words used so far
+      for (int64_t t = first; t < total; t += step, ++i) {
+        if (i > 0 && !mbar_wait_cluster(tempty, (i - 1) & 1, abort_flag, p.err)) {
+          st_cluster_u32(peer_abort, 1);
+          goto out;
+        }
+        tc_fence_after();
+        const uint32_t acc = tmem + ((i & 1) ? Cfg::ACC1 : 0u);
+        for (int kb = 0; kb < p.num_kb; ++kb) {
+          const uint32_t sf = tmem + Cfg::SF + (u & 1) * 12;
+          if ((kb & 3) == 0) {
+            if (!mbar_wait_cluster(&sf_full[u & 1], (u >> 1) & 1, abort_flag, p.err)) {
+              st_cluster_u32(peer_abort, 1);
+              goto out;
+            }
+            tc_fence_after();
+            const uint32_t src = smem_u32(sSF + (u & 1) * Cfg::SF_BYTES);
+            tmem_copy_scales_pair(sf, sdesc_rows16(src));
+            tmem_copy_scales_pair(sf + 4, sdesc_rows16(src + 512));
+            tmem_copy_scales_pair(sf + 8, sdesc_rows16(src + 1024));
+          }
+          if (!mbar_wait_cluster(&full[s], ph, abort_flag, p.err)) {
+            st_cluster_u32(peer_abort, 1);
+            goto out;
+          }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(sA + s * Cfg::HALF_BYTES);
+          const uint32_t w0 = smem_u32(sW + s * Cfg::HALF_BYTES);
+          const uint32_t id = idesc_with_scale_byte(idesc, kb & 3);
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / 32; ++kk)
+            umma_e4m3_scaled_pair(acc, sdesc_sw128(a0 + kk * 32, 16, 1024),
+                                  sdesc_sw128(w0 + kk * 32, 16, 1024), id, sf, sf + 4,
+                                  (kb | kk) ? 1u : 0u);
+          umma_commit_pair(&empty[s], 0x3);
+          if ((kb & 3) == 3 || kb + 1 == p.num_kb) {
+            umma_commit_pair(&sf_empty[u & 1], 0x3);
+            ++u;
+          }
+          if (++s == Cfg::STAGES) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        umma_commit_pair(&tfull[i & 1], 0x3);
+      }
+    }
+  } else if (warp == 2) {
+    // scale words of 512 of K: row lane + 32 j of the tile to word j of row `lane`
+    const uint32_t sf_full_lead = cluster_addr(sf_full, 0);
+    const int groups = (p.num_kb + 3) >> 2;
+    uint32_t u = 0;
+    for (int64_t t = first; t < total; t += step) {
+      const int64_t m0 = (t / p.tiles_n) * 256 + rank * 128;
+      const int n0 = (int)(t % p.tiles_n) * 256;
+      for (int g = 0; g < groups; ++g, ++u) {
+        uint32_t a[4], w[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int64_t m = m0 + lane + 32 * j;
+          a[j] = m < p.M ? __ldg(p.a_scales + (int64_t)g * p.M + m) : 0x7f7f7f7fu;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int n = n0 + lane + 32 * j;
+          w[j] = n < p.N ? __ldg(p.w_scales + (int64_t)g * p.N + n) : 0x7f7f7f7fu;
+        }
+        const bool ok = mbar_wait_cluster(&sf_empty[u & 1], ((u >> 1) & 1) ^ 1, abort_flag, p.err);
+        if (!__all_sync(0xffffffffu, ok)) {
+          if (lane == 0) st_cluster_u32(peer_abort, 1);
+          goto out;
+        }
+        uint4* dst = reinterpret_cast<uint4*>(sSF + (u & 1) * Cfg::SF_BYTES);
+        dst[lane] = make_uint4(a[0], a[1], a[2], a[3]);
+        dst[32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+        dst[64 + lane] = make_uint4(w[4], w[5], w[6], w[7]);
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(sf_full_lead + (u & 1) * 8);
+      }
+    }
+  } else {
+    // Epilogue: TMEM lanes of `quarter`, 128 columns of `half`, 64 at a time, the half's
+    // end that overlaps the other accumulator first (columns 232.. of the first, 0..23
+    // of the second).
+    const int quarter = warp & 3, half = (warp - 3) >> 2;
+    uint8_t* box = sOut + (warp - 3) * 4096;
+    const uint32_t tempty_lead = cluster_addr(tempty, 0);
+    int i = 0;
+    for (int64_t t = first; t < total; t += step, ++i) {
+      const int64_t row0 = (t / p.tiles_n) * 256 + rank * 128 + quarter * 32;
+      const int n0 = (int)(t % p.tiles_n) * 256;
+      const bool overlaps = half != (i & 1);         // this half reads the overlap
+      if (!overlaps && lane == 0) mbar_arrive_cluster(tempty_lead);
+      const bool ok = mbar_wait_cluster(&tfull[i & 1], (i >> 1) & 1, abort_flag, p.err);
+      if (!__all_sync(0xffffffffu, ok)) {
+        if (lane == 0) st_cluster_u32(peer_abort, 1);
+        goto out;
+      }
+      tc_fence_after();
+      const uint32_t tacc =
+          tmem + ((i & 1) ? Cfg::ACC1 : 0u) + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+      for (int gi = 0; gi < 2; ++gi) {
+        const int c64 = half ? 192 - 64 * gi : 64 * gi;
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi) {
+          const int h = half ? 1 - hi : hi;
+          uint32_t v[32], w[16];
+          tmem_ld_32x32b_x32(tacc + c64 + h * 32, v);
+          tmem_ld_wait();
+          if (overlaps && gi == 0 && hi == 0) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(tempty_lead);
+          }
+          finish32(p, v, row0 + lane, n0 + c64 + h * 32, w);
+          if (hi == 0) {                             // the last store has read the box
+            if (lane == 0) bulk_wait_read_all();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *reinterpret_cast<uint4*>(box + lane * 128 + (((h * 4 + j) ^ (lane & 7)) * 16)) =
+                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0 && row0 < p.M && n0 + c64 < p.N) {
+          tma_store_3d(&tmC, box, n0 + c64, (int)row0, 0);
+          bulk_commit_group();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+
+out:
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();            // no CTA leaves while the other may still use it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+std::atomic<int> g_pairs{0};   // pairs resident at once, 0 until the kernel is loaded
+
+int launch_pair(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
+  const uint64_t pitch = (uint64_t)e4m3_pitch(g.K);
+  CUtensorMap ta, tw, tc;
+  if (!make_tmap_2d_u8(&ta, g.a, pitch, (uint64_t)g.M, 128) ||
+      !make_tmap_2d_u8(&tw, g.w, pitch, (uint64_t)g.N, 128) ||
+      !make_tmap_3d_f16(&tc, g.out, (uint64_t)g.N, (uint64_t)g.M, 1, 64, 32))
+    return HEXLIB_B200_ERR_CUDA;
+  E4m3Params p = params_of(g, err);
+  p.tiles_n = (g.N + 255) / 256;
+  const int64_t tiles = (int64_t)((g.M + 255) / 256) * p.tiles_n;
+  const int64_t pairs = g_pairs.load(std::memory_order_relaxed);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)), 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = cluster_of(attr, 2);
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, gemm_e4m3_pair, ta, tw, tc, p) != cudaSuccess) {
+    cudaGetLastError();
+    return HEXLIB_B200_ERR_CUDA;
+  }
+  return HEXLIB_B200_OK;
+}
+
+// What the pair kernel asks of the output: whole 16-byte vectors in every row.
+bool pair_can(const GemmE4m3Desc& g) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.resid) |
+                         reinterpret_cast<uintptr_t>(g.bias) | static_cast<uintptr_t>(2) * g.N;
+  return bits % 16 == 0 && g_pairs.load(std::memory_order_relaxed) > 0;
 }
 
 }  // namespace
@@ -291,14 +641,31 @@ int gemm_e4m3_kernels_init() {
       cudaFuncSetAttribute(gemm_e4m3_tile<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            TileCfg<64>::SMEM_BYTES) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_e4m3_tile<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           TileCfg<128>::SMEM_BYTES) != cudaSuccess) {
+                           TileCfg<128>::SMEM_BYTES) != cudaSuccess ||
+      cudaFuncSetAttribute(gemm_e4m3_pair, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           PairCfg::SMEM_BYTES) != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(512, 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = cluster_of(attr, 2);
+  cfg.numAttrs = 1;
+  int pairs = 0;
+  if (cudaOccupancyMaxActiveClusters(&pairs, gemm_e4m3_pair, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return HEXLIB_B200_ERR_CUDA;
+  }
+  g_pairs.store(pairs, std::memory_order_relaxed);
   return HEXLIB_B200_OK;
 }
 
 int launch_gemm_e4m3(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
+  if (g.M > 256 && (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) >= 37 && pair_can(g))
+    return launch_pair(g, err, s);
   const int num_kb = (int)(e4m3_pitch(g.K) / kBlockK);
   const int bn = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   const int64_t tiles = (int64_t)((g.N + 127) / 128) * ((g.M + bn - 1) / bn);

@@ -241,3 +241,24 @@ def test_empty_batches_launch_nothing():
     assert U.call_rc("hexlib_b200_quantize_e4m3_fp16", None, None, None, 0, 64, U.stream()) == U.OK
     assert U.call_rc("hexlib_b200_matmul_epilogue_e4m3", None, None, None, None, None, None, 0, 64, 64, 0,
                      U.stream()) == U.OK
+
+
+# outputs of many 256 x 256 tiles, several to a pair of SMs, with ragged edges in every
+# direction and each epilogue
+@pytest.mark.parametrize("M,K,N,act,with_bias,with_resid", [
+    (2500, 513, 1000, 0, False, False), (4097, 1100, 1032, 0, True, True), (9000, 300, 1288, 1, True, False),
+    (9473, 640, 520, 1, False, True), (5000, 128, 2048, 0, True, False), (3000, 2100, 1536, 2, True, True),
+    (19000, 1, 264, 0, False, False), (20000, 260, 512, 0, False, False)])
+def test_product_of_many_tiles(M, K, N, act, with_bias, with_resid):
+    rng = np.random.default_rng(M + K)
+    a, w = operands(rng, M, K, N, spread=3)
+    bias = rng.standard_normal(N).astype(np.float32) if with_bias else None
+    resid = rng.standard_normal((M, N)).astype(np.float16) if with_resid else None
+    ref, bound = B.product(a[2], w[2], bias, resid, act)
+    y = U.dev(resid) if with_resid else U.empty((M, N), np.float16)
+    product(a, w, M, K, N, act, bias, y if with_resid else None, out=y)
+    first = U.host(y)
+    B.assert_within(first, ref, bound, "tiles")
+    if not with_resid:
+        product(a, w, M, K, N, act, bias, None, out=y)
+        assert np.array_equal(first, U.host(y))
