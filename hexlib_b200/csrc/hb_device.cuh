@@ -128,6 +128,19 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
   return mbar_wait_limit(bar, parity, abort_flag, err, HB_WAIT_LIMIT_NS);
 }
 
+// ---- programmatic serialization ---------------------------------------------
+// A kernel that calls grid_dependents_may_start lets the next one in its stream start
+// (where that was launched to allow it) as soon as every CTA has called it or ended;
+// grid_dependency_wait returns once the kernel before has finished and its writes are
+// visible. Neither does anything in an ordinary launch.
+
+__device__ __forceinline__ void grid_dependents_may_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void grid_dependency_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ---- CTA pairs (clusters of two; see gemm_f16_pair) ------------------------
 
 __device__ __forceinline__ uint32_t cluster_ctarank() {
@@ -143,17 +156,19 @@ __device__ __forceinline__ void cluster_sync() {
                "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The two halves of cluster_sync, for work in between.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Address of the same shared-memory object in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
-}
-
-__device__ __forceinline__ float ld_cluster_f32(uint32_t caddr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(caddr) : "memory");
-  return v;
 }
 
 __device__ __forceinline__ void st_cluster_u32(uint32_t caddr, uint32_t v) {
@@ -191,6 +206,29 @@ __device__ __forceinline__ bool mbar_try_wait_cluster_suspend(uint64_t* bar, uin
   return ok != 0;
 }
 
+// ---- warp-uniform issue ------------------------------------------------------
+// tcgen05 and TMA instructions take their descriptors from uniform registers. A role
+// whose whole warp runs its loop, with one elected lane issuing, keeps them there;
+// a loop under `lane == 0` moves each operand over at every issue.
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(p));
+  return p != 0;
+}
+
+// The waits of a whole warp (the same answer in every lane).
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity,
+                                               volatile int* abort_flag, int* err) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu,
+                    mbar_wait_limit(bar, parity, abort_flag, err, HB_WAIT_LIMIT_NS));
+}
+
 // mbar_wait with cluster-scope acquire, for barriers arrived on from the
 // other CTA of a pair. Same limit and abort protocol as mbar_wait_limit.
 __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity,
@@ -206,6 +244,12 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
       return false;
     }
   }
+}
+
+__device__ __forceinline__ bool mbar_wait_cluster_warp(uint64_t* bar, uint32_t parity,
+                                                       volatile int* abort_flag, int* err) {
+  if (__all_sync(0xffffffffu, mbar_try_wait_cluster(bar, parity))) return true;
+  return __all_sync(0xffffffffu, mbar_wait_cluster(bar, parity, abort_flag, err));
 }
 
 // ---- TMA (no multicast anywhere in this project) ---------------------------
@@ -241,6 +285,12 @@ __device__ __forceinline__ void tma_prefetch_l2_3d(const CUtensorMap* map, int c
                                                    int c2) {
   asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];"
                ::"l"(map), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+
+__device__ __forceinline__ void tma_prefetch_l2_2d(const CUtensorMap* map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map),
+               "r"(c0), "r"(c1)
                : "memory");
 }
 

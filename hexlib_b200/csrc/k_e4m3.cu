@@ -2,6 +2,7 @@
 // activations and weights of the 8-bit matrix product (k_gemm_e4m3.cu).
 #include <cuda_runtime.h>
 
+#include "hb_device.cuh"
 #include "hb_e4m3.cuh"
 #include "hb_kernels.h"
 
@@ -23,6 +24,7 @@ __global__ void __launch_bounds__(kThreads) quantize_e4m3(const __half* __restri
                                                           uint8_t* __restrict__ codes,
                                                           uint32_t* __restrict__ scales,
                                                           int64_t R, int K) {
+  grid_dependents_may_start();         // the product that follows waits for the codes itself
   const int l = threadIdx.x & 15;
   const uint32_t half_mask = 0xffffu << (threadIdx.x & 16);
   const int blocks = (K + 127) / 128, groups = (blocks + 3) / 4;

@@ -51,23 +51,32 @@ __device__ __forceinline__ float finish(float v, int act) {
 // any alignment of the output.
 //
 // A cluster of S CTAs shares a tile and splits K: with few tokens the time is that
-// of reading w once, which takes all SMs. Each CTA leaves its partial tile in its
-// shared memory, and CTA r adds up its BN / S tokens from all of them, in rank order.
+// of reading w once, which takes all SMs. Each CTA sends the partial sums of BN / S
+// tokens to each of the others' shared memory, and adds up what it was sent in rank
+// order, so the result does not depend on who was first.
+//
+// Launched with programmatic serialization: a CTA may start while the kernel before
+// (the quantization of a, which lets it) is still running. Until that has finished it
+// only sets up and brings its part of w to L2, which is right whoever wrote w last.
 template <int BN>
 struct TileCfg {
   static constexpr int W_BYTES = 128 * kBlockK;
   static constexpr int A_BYTES = BN * kBlockK;
   static constexpr int STAGE_BYTES = W_BYTES + A_BYTES;
-  static constexpr int STAGES = BN == 128 ? 3 : 4;
+  static constexpr int STAGES = 4;
   static constexpr int SF_BYTES = 2 * 2 * 512;                    // two buffers of w and a
+  static constexpr int PART_BYTES = BN * 128 * 4;                 // sums from the other ranks
   static constexpr int TMEM_COLS = BN == 16 ? 32 : 2 * BN;        // accumulator + 16 of scales
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SF_BYTES + 1024 + 256;
+  static constexpr int smem(int split) {
+    return STAGES * STAGE_BYTES + SF_BYTES + (split > 1 ? PART_BYTES : 0) + 1024 + 256;
+  }
 };
 
 template <int BN>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     gemm_e4m3_tile(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA,
-                   const E4m3Params p, const int split) {
+                   const E4m3Params p, const int split_log2) {
+  const int split = 1 << split_log2;
   using Cfg = TileCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -75,7 +84,9 @@ __global__ void __launch_bounds__(kThreads)
   uint8_t* sW = smem;
   uint8_t* sA = smem + Cfg::STAGES * Cfg::W_BYTES;
   uint8_t* sSF = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + Cfg::SF_BYTES);
+  float* part = reinterpret_cast<float*>(sSF + Cfg::SF_BYTES);   // [split][BN / split][128]
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + Cfg::SF_BYTES +
+                                               (split > 1 ? Cfg::PART_BYTES : 0));
   uint64_t* empty = full + Cfg::STAGES;
   uint64_t* sf_full = empty + Cfg::STAGES;
   uint64_t* sf_empty = sf_full + 2;
@@ -83,8 +94,16 @@ __global__ void __launch_bounds__(kThreads)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
+  const int tile = blockIdx.x / split;
+  const int n0 = (tile % p.tiles_n) * 128, m0 = (tile / p.tiles_n) * BN;
+  // the blocks of K of this CTA (at least one: split <= num_kb)
+  const int kb0 = (int)((int64_t)p.num_kb * rank / split);
+  const int kb1 = (int)((int64_t)p.num_kb * (rank + 1) / split);
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmA);
     for (int s = 0; s < Cfg::STAGES; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
@@ -96,8 +115,8 @@ __global__ void __launch_bounds__(kThreads)
     mbar_init(done, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmA);
+  } else if (warp == 3 && lane == 0) {
+    for (int kb = kb0; kb < kb1 && kb < kb0 + 8; ++kb) tma_prefetch_l2_2d(&tmW, kb * kBlockK, n0);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
@@ -106,54 +125,72 @@ __global__ void __launch_bounds__(kThreads)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  if (split > 1) cluster_arrive();                   // waited for before the parts are sent
+  grid_dependency_wait();
 
-  const int rank = split > 1 ? (int)cluster_ctarank() : 0;
-  const int tile = blockIdx.x / split;
-  const int n0 = (tile % p.tiles_n) * 128, m0 = (tile / p.tiles_n) * BN;
-  // the blocks of K of this CTA (at least one: split <= num_kb)
-  const int kb0 = (int)((int64_t)p.num_kb * rank / split);
-  const int kb1 = (int)((int64_t)p.num_kb * (rank + 1) / split);
-
-  if (warp == 0 && lane == 0) {
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const int i = kb - kb0, s = i % Cfg::STAGES;
-      if (!mbar_wait(&empty[s], ((i / Cfg::STAGES) & 1) ^ 1, abort_flag, p.err)) break;
-      mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES);
-      tma_load_2d(&tmW, &full[s], sW + s * Cfg::W_BYTES, kb * kBlockK, n0);
-      tma_load_2d(&tmA, &full[s], sA + s * Cfg::A_BYTES, kb * kBlockK, m0);
-    }
-  } else if (warp == 1 && lane == 0) {
-    constexpr uint32_t idesc = idesc_e4m3_scaled(128, BN);
-    int u = 0;                                        // scale words used so far
-    bool ok = true;
-    for (int kb = kb0; kb < kb1 && ok; ++kb) {
-      const int i = kb - kb0, s = i % Cfg::STAGES;
-      const uint32_t sf = tmem + BN + (u & 1) * 8;
-      if (i == 0 || (kb & 3) == 0) {
-        ok = mbar_wait(&sf_full[u & 1], (u >> 1) & 1, abort_flag, p.err);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t src = smem_u32(sSF + (u & 1) * 1024);
-        tmem_copy_scales(sf, sdesc_rows16(src));
-        tmem_copy_scales(sf + 4, sdesc_rows16(src + 512));
-      }
-      ok = mbar_wait(&full[s], (i / Cfg::STAGES) & 1, abort_flag, p.err);
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t w0 = smem_u32(sW + s * Cfg::W_BYTES), a0 = smem_u32(sA + s * Cfg::A_BYTES);
-      const uint32_t id = idesc_with_scale_byte(idesc, kb & 3);
+  // The loops over blocks of K go round the ring of stages, whose addresses are then
+  // constants of the code: with addresses, descriptors and branches formed anew for
+  // each block by one lane, a block took 400 ns to issue, more than its loads.
+  if (warp == 0) {
+    int kb = kb0;
+    for (uint32_t ph = 1; kb < kb1; ph ^= 1u) {
 #pragma unroll
-      for (int kk = 0; kk < kBlockK / 32; ++kk)
-        umma_e4m3_scaled(tmem, sdesc_sw128(w0 + kk * 32, 16, 1024),
-                         sdesc_sw128(a0 + kk * 32, 16, 1024), id, sf, sf + 4, (i | kk) ? 1u : 0u);
-      umma_commit(&empty[s]);
-      if ((kb & 3) == 3 || kb + 1 == kb1) {
-        umma_commit(&sf_empty[u & 1]);
-        ++u;
+      for (int s = 0; s < Cfg::STAGES; ++s) {
+        if (kb >= kb1) break;
+        if (!mbar_wait_warp(&empty[s], ph, abort_flag, p.err)) {
+          kb = kb1;
+          break;
+        }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES);
+          tma_load_2d(&tmW, &full[s], sW + s * Cfg::W_BYTES, kb * kBlockK, n0);
+          tma_load_2d(&tmA, &full[s], sA + s * Cfg::A_BYTES, kb * kBlockK, m0);
+        }
+        ++kb;
       }
     }
-    if (ok) umma_commit(done);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = idesc_e4m3_scaled(128, BN);
+    const uint64_t dw = sdesc_sw128(smem_u32(sW), 16, 1024);
+    const uint64_t da = sdesc_sw128(smem_u32(sA), 16, 1024);
+    const uint64_t dsf = sdesc_rows16(smem_u32(sSF));
+    uint32_t u = 0;                                   // scale words used so far
+    int kb = kb0;
+    bool ok = true;
+    for (uint32_t ph = 0; kb < kb1; ph ^= 1u) {
+#pragma unroll
+      for (int s = 0; s < Cfg::STAGES; ++s) {
+        if (kb >= kb1) break;
+        const uint32_t b = u & 1, sf = tmem + BN + b * 8;
+        const bool fresh = kb == kb0 || (kb & 3) == 0;
+        if (fresh) ok = mbar_wait_warp(&sf_full[b], (u >> 1) & 1, abort_flag, p.err);
+        ok = ok && mbar_wait_warp(&full[s], ph, abort_flag, p.err);
+        if (!ok) {
+          kb = kb1;
+          break;
+        }
+        tc_fence_after();
+        const bool last_of_word = (kb & 3) == 3 || kb + 1 == kb1;
+        if (elect_one()) {
+          if (fresh) {
+            tmem_copy_scales(sf, dsf + b * (1024 >> 4));
+            tmem_copy_scales(sf + 4, dsf + b * (1024 >> 4) + (512 >> 4));
+          }
+          const uint32_t id = idesc_with_scale_byte(idesc, kb & 3);
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / 32; ++kk)
+            umma_e4m3_scaled(tmem, dw + (s * Cfg::W_BYTES + kk * 32 >> 4),
+                             da + (s * Cfg::A_BYTES + kk * 32 >> 4), id, sf, sf + 4,
+                             kk > 0 || kb > kb0 ? 1u : 0u);
+          umma_commit(&empty[s]);
+          if (last_of_word) umma_commit(&sf_empty[b]);
+        }
+        u += last_of_word;
+        ++kb;
+      }
+    }
+    if (ok && elect_one()) umma_commit(done);
   } else if (warp == 2) {
     // scale words of 512 of K: row lane + 32 j of the tile to word j of row `lane`
     int u = 0;
@@ -187,6 +224,7 @@ __global__ void __launch_bounds__(kThreads)
   constexpr int CH = COLS < 32 ? COLS : 32;          // of them at a time
   const uint32_t tacc = tmem + ((uint32_t)(quarter * 32) << 16) + half * COLS;
   const int n = n0 + quarter * 32 + lane;
+  if (split > 1) cluster_wait();                     // every rank has started
 #pragma unroll
   for (int c0 = 0; c0 < COLS; c0 += CH) {
     if (!ok) break;
@@ -196,10 +234,15 @@ __global__ void __launch_bounds__(kThreads)
     else tmem_ld_32x32b_x32(tacc + c0, v);
     tmem_ld_wait();
     if (split > 1) {
-      float* part = reinterpret_cast<float*>(smem);  // [BN][128]; every load has been used
+      // token c goes to rank c / cols, at [this rank][c % cols][feature] there
+      constexpr int BN_LOG2 = BN == 16 ? 4 : BN == 32 ? 5 : BN == 64 ? 6 : 7;
+      const int cols_log2 = BN_LOG2 - split_log2, cols = 1 << cols_log2;
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-        part[(half * COLS + c0 + c) * 128 + quarter * 32 + lane] = __uint_as_float(v[c]);
+      for (int c = 0; c < CH; ++c) {
+        const int tok = half * COLS + c0 + c;
+        float* to = part + ((rank << cols_log2) + (tok & (cols - 1))) * 128 + quarter * 32 + lane;
+        st_cluster_u32(cluster_addr(to, tok >> cols_log2), v[c]);
+      }
     } else if (n < p.N) {
       const float bias = p.bias ? __ldg(p.bias + n) : 0.f;
       const int m = m0 + half * COLS + c0;
@@ -217,22 +260,20 @@ __global__ void __launch_bounds__(kThreads)
   }
   if (split > 1) {
     tc_fence_before();
-    cluster_sync();
-    const int cols = BN / split;                     // tokens this CTA finishes
+    cluster_sync();                                  // every rank's part has arrived
+    const int cols = BN >> split_log2;               // tokens this CTA finishes
     const int f = threadIdx.x & 127;
     const bool in_n = n0 + f < p.N;
     const float bias = p.bias && in_n ? __ldg(p.bias + n0 + f) : 0.f;
-    for (int c = rank * cols + (threadIdx.x >> 7); c < (rank + 1) * cols; c += kThreads / 128) {
-      const int m = m0 + c;
+    for (int c = threadIdx.x >> 7; c < cols; c += kThreads / 128) {
+      const int m = m0 + rank * cols + c;
       if (m >= p.M || !in_n) continue;
       const int64_t o = (int64_t)m * p.N + n0 + f;
       const float r = p.resid ? __half2float(p.resid[o]) : 0.f;
-      const float* mine = reinterpret_cast<const float*>(smem) + c * 128 + f;
       float v = 0.f;
-      for (int q = 0; q < split; ++q) v += ld_cluster_f32(cluster_addr(mine, q));
+      for (int q = 0; q < split; ++q) v += part[(q * cols + c) * 128 + f];
       p.out[o] = __float2half_rn(finish(v + bias, p.act) + r);
     }
-    cluster_sync();                                  // until the others have read this CTA's part
   }
   tc_fence_before();
   __syncthreads();
@@ -266,7 +307,8 @@ cudaLaunchAttribute* cluster_of(cudaLaunchAttribute* attr, int n) {
 }
 
 template <int BN>
-int launch_tile(const GemmE4m3Desc& g, int split, int* err, cudaStream_t s) {
+int launch_tile(const GemmE4m3Desc& g, int split_log2, int* err, cudaStream_t s) {
+  const int split = 1 << split_log2;
   using Cfg = TileCfg<BN>;
   const uint64_t pitch = (uint64_t)e4m3_pitch(g.K);
   CUtensorMap tw, ta;
@@ -280,12 +322,14 @@ int launch_tile(const GemmE4m3Desc& g, int split, int* err, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * split), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
-  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.dynamicSmemBytes = Cfg::smem(split);
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.attrs = cluster_of(attr, split);
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, gemm_e4m3_tile<BN>, tw, ta, p, split) != cudaSuccess) {
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
+  if (cudaLaunchKernelEx(&cfg, gemm_e4m3_tile<BN>, tw, ta, p, split_log2) != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
@@ -389,7 +433,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   if (threadIdx.x == 0) {
     for (int s = 0; s < Cfg::STAGES; ++s) {
@@ -415,84 +459,96 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const uint32_t peer_abort = cluster_addr(tmem_slot + 1, rank ^ 1u);
+  grid_dependency_wait();
 
   const int64_t total = (int64_t)((p.M + 255) / 256) * p.tiles_n;
   const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
+  // (loops round the ring of stages, as in the tile kernel, through all tiles)
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t full_lead = cluster_addr(full, 0);
-      int s = 0;
-      uint32_t ph = 0;
-      for (int64_t t = first; t < total; t += step) {
-        const int row = (int)(t / p.tiles_n) * 256 + (int)rank * 128;
-        const int col = (int)(t % p.tiles_n) * 256 + (int)rank * 128;
-        for (int kb = 0; kb < p.num_kb; ++kb) {
-          if (!mbar_wait_cluster(&empty[s], ph ^ 1u, abort_flag, p.err)) {
-            st_cluster_u32(peer_abort, 1);
-            goto out;
-          }
+    const uint32_t full_lead = cluster_addr(full, 0);
+    int64_t t = first;
+    int kb = 0;
+    int row = (int)(t / p.tiles_n) * 256 + (int)rank * 128;
+    int col = (int)(t % p.tiles_n) * 256 + (int)rank * 128;
+    for (uint32_t ph = 1; t < total; ph ^= 1u) {
+#pragma unroll
+      for (int s = 0; s < Cfg::STAGES; ++s) {
+        if (t >= total) break;
+        if (!mbar_wait_cluster_warp(&empty[s], ph, abort_flag, p.err)) {
+          if (lane == 0) st_cluster_u32(peer_abort, 1);
+          t = total;
+          break;
+        }
+        if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE_BYTES);
           tma_load_2d_pair(&tmA, full_lead + s * 8, sA + s * Cfg::HALF_BYTES, kb * kBlockK, row);
           tma_load_2d_pair(&tmW, full_lead + s * 8, sW + s * Cfg::HALF_BYTES, kb * kBlockK, col);
-          if (++s == Cfg::STAGES) {
-            s = 0;
-            ph ^= 1u;
-          }
+        }
+        if (++kb == p.num_kb) {
+          kb = 0;
+          t += step;
+          row = (int)(t / p.tiles_n) * 256 + (int)rank * 128;
+          col = (int)(t % p.tiles_n) * 256 + (int)rank * 128;
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       constexpr uint32_t idesc = idesc_e4m3_scaled(256, 256);
-      int s = 0, i = 0;
-      uint32_t ph = 0, u = 0;                        // u: scale words used so far
-      for (int64_t t = first; t < total; t += step, ++i) {
-        if (i > 0 && !mbar_wait_cluster(tempty, (i - 1) & 1, abort_flag, p.err)) {
-          st_cluster_u32(peer_abort, 1);
-          goto out;
-        }
-        tc_fence_after();
-        const uint32_t acc = tmem + ((i & 1) ? Cfg::ACC1 : 0u);
-        for (int kb = 0; kb < p.num_kb; ++kb) {
-          const uint32_t sf = tmem + Cfg::SF + (u & 1) * 12;
-          if ((kb & 3) == 0) {
-            if (!mbar_wait_cluster(&sf_full[u & 1], (u >> 1) & 1, abort_flag, p.err)) {
-              st_cluster_u32(peer_abort, 1);
-              goto out;
-            }
-            tc_fence_after();
-            const uint32_t src = smem_u32(sSF + (u & 1) * Cfg::SF_BYTES);
-            tmem_copy_scales_pair(sf, sdesc_rows16(src));
-            tmem_copy_scales_pair(sf + 4, sdesc_rows16(src + 512));
-            tmem_copy_scales_pair(sf + 8, sdesc_rows16(src + 1024));
-          }
-          if (!mbar_wait_cluster(&full[s], ph, abort_flag, p.err)) {
-            st_cluster_u32(peer_abort, 1);
-            goto out;
+      const uint64_t da = sdesc_sw128(smem_u32(sA), 16, 1024);
+      const uint64_t dw = sdesc_sw128(smem_u32(sW), 16, 1024);
+      const uint64_t dsf = sdesc_rows16(smem_u32(sSF));
+      uint32_t u = 0, i = 0;                         // scale words, tiles so far
+      int64_t t = first;
+      int kb = 0;
+      for (uint32_t ph = 0; t < total; ph ^= 1u) {
+#pragma unroll
+        for (int s = 0; s < Cfg::STAGES; ++s) {
+          if (t >= total) break;
+          const uint32_t b = u & 1, sf = tmem + Cfg::SF + b * 12;
+          const uint32_t acc = tmem + ((i & 1) ? Cfg::ACC1 : 0u);
+          const bool fresh = (kb & 3) == 0;
+          bool ok = true;
+          if (kb == 0 && i > 0)
+            ok = mbar_wait_cluster_warp(tempty, (i - 1) & 1, abort_flag, p.err);
+          if (fresh)
+            ok = ok && mbar_wait_cluster_warp(&sf_full[b], (u >> 1) & 1, abort_flag, p.err);
+          ok = ok && mbar_wait_cluster_warp(&full[s], ph, abort_flag, p.err);
+          if (!ok) {
+            if (lane == 0) st_cluster_u32(peer_abort, 1);
+            t = total;
+            break;
           }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(sA + s * Cfg::HALF_BYTES);
-          const uint32_t w0 = smem_u32(sW + s * Cfg::HALF_BYTES);
-          const uint32_t id = idesc_with_scale_byte(idesc, kb & 3);
+          const bool last = kb + 1 == p.num_kb;
+          const bool last_of_word = last || (kb & 3) == 3;
+          if (elect_one()) {
+            if (fresh) {
+              tmem_copy_scales_pair(sf, dsf + b * (Cfg::SF_BYTES >> 4));
+              tmem_copy_scales_pair(sf + 4, dsf + b * (Cfg::SF_BYTES >> 4) + (512 >> 4));
+              tmem_copy_scales_pair(sf + 8, dsf + b * (Cfg::SF_BYTES >> 4) + (1024 >> 4));
+            }
+            const uint32_t id = idesc_with_scale_byte(idesc, kb & 3);
 #pragma unroll
-          for (int kk = 0; kk < kBlockK / 32; ++kk)
-            umma_e4m3_scaled_pair(acc, sdesc_sw128(a0 + kk * 32, 16, 1024),
-                                  sdesc_sw128(w0 + kk * 32, 16, 1024), id, sf, sf + 4,
-                                  (kb | kk) ? 1u : 0u);
-          umma_commit_pair(&empty[s], 0x3);
-          if ((kb & 3) == 3 || kb + 1 == p.num_kb) {
-            umma_commit_pair(&sf_empty[u & 1], 0x3);
-            ++u;
+            for (int kk = 0; kk < kBlockK / 32; ++kk)
+              umma_e4m3_scaled_pair(acc, da + (s * Cfg::HALF_BYTES + kk * 32 >> 4),
+                                    dw + (s * Cfg::HALF_BYTES + kk * 32 >> 4), id, sf, sf + 4,
+                                    kk > 0 || kb > 0 ? 1u : 0u);
+            umma_commit_pair(&empty[s], 0x3);
+            if (last_of_word) umma_commit_pair(&sf_empty[b], 0x3);
+            if (last) umma_commit_pair(&tfull[i & 1], 0x3);
           }
-          if (++s == Cfg::STAGES) {
-            s = 0;
-            ph ^= 1u;
+          u += last_of_word;
+          ++kb;
+          if (last) {
+            kb = 0;
+            t += step;
+            ++i;
           }
         }
-        umma_commit_pair(&tfull[i & 1], 0x3);
       }
     }
   } else if (warp == 2) {
@@ -614,9 +670,11 @@ int launch_pair(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
   cfg.blockDim = dim3(kPairThreads, 1, 1);
   cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   cfg.attrs = cluster_of(attr, 2);
-  cfg.numAttrs = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, gemm_e4m3_pair, ta, tw, tc, p) != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
@@ -635,13 +693,13 @@ bool pair_can(const GemmE4m3Desc& g) {
 
 int gemm_e4m3_kernels_init() {
   if (cudaFuncSetAttribute(gemm_e4m3_tile<16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           TileCfg<16>::SMEM_BYTES) != cudaSuccess ||
+                           TileCfg<16>::smem(2)) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_e4m3_tile<32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           TileCfg<32>::SMEM_BYTES) != cudaSuccess ||
+                           TileCfg<32>::smem(2)) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_e4m3_tile<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           TileCfg<64>::SMEM_BYTES) != cudaSuccess ||
+                           TileCfg<64>::smem(2)) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_e4m3_tile<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           TileCfg<128>::SMEM_BYTES) != cudaSuccess ||
+                           TileCfg<128>::smem(2)) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_e4m3_pair, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            PairCfg::SMEM_BYTES) != cudaSuccess) {
     cudaGetLastError();
@@ -669,8 +727,8 @@ int launch_gemm_e4m3(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
   const int num_kb = (int)(e4m3_pitch(g.K) / kBlockK);
   const int bn = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   const int64_t tiles = (int64_t)((g.N + 127) / 128) * ((g.M + bn - 1) / bn);
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= 296 && num_kb >= split * 4) split *= 2;
+  int split = 0;
+  while (split < 3 && (tiles << (split + 1)) <= 296 && num_kb >= 4 << split) ++split;
   switch (bn) {
     case 16: return launch_tile<16>(g, split, err, s);
     case 32: return launch_tile<32>(g, split, err, s);
