@@ -364,19 +364,21 @@ struct PairCfg {
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;      // of each CTA
   static constexpr int SF_BYTES = 512 + 1024;             // own rows of a, all rows of w
   static constexpr int STAGING = 8 * 4096;                // a 32 x 64 fp16 box per warp
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + STAGING + 2 * SF_BYTES + 1024 + 256;
+  static constexpr int BIAS_BYTES = 8 * 512;              // the 128 columns of each
+  static constexpr int SMEM_BYTES =
+      STAGES * STAGE_BYTES + STAGING + 2 * SF_BYTES + BIAS_BYTES + 1024 + 256;
   static constexpr uint32_t ACC1 = 232, SF = 488;
 };
 
-// 32 columns of a row: bias, activation, residual, one rounding.
+// 32 columns of a row: bias (its 32 values in shared memory), activation, residual, one
+// rounding.
 __device__ __forceinline__ void finish32(const E4m3Params& p, uint32_t (&v)[32], int64_t row,
-                                         int n, uint32_t (&w)[16]) {
+                                         int n, const float* bias, uint32_t (&w)[16]) {
   const bool row_ok = row < p.M;
   if (p.bias) {
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-      const float4 b = n + j < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + n + j))
-                                   : make_float4(0, 0, 0, 0);
+      const float4 b = *reinterpret_cast<const float4*>(bias + j);
       v[j] = __float_as_uint(__uint_as_float(v[j]) + b.x);
       v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + b.y);
       v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) + b.z);
@@ -413,6 +415,31 @@ __device__ __forceinline__ void finish32(const E4m3Params& p, uint32_t (&v)[32],
     w[q] = pack_half2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
 }
 
+// The tiles of a CTA pair, `step` apart in row-major order, without a division between
+// them (the 64-bit ones of the direct form took a tenth of a short tile's time).
+struct TileWalk {
+  uint32_t m, n, left;                               // tile coordinates, tiles still to do
+  uint32_t dm, dn, tiles_n;
+  __device__ TileWalk(uint32_t tiles_m, uint32_t tiles_n_, uint32_t first, uint32_t step)
+      : tiles_n(tiles_n_) {
+    const uint32_t total = tiles_m * tiles_n;
+    m = first / tiles_n;
+    n = first - m * tiles_n;
+    dm = step / tiles_n;
+    dn = step - dm * tiles_n;
+    left = first < total ? (total - first + step - 1) / step : 0;
+  }
+  __device__ void next() {
+    --left;
+    m += dm;
+    n += dn;
+    if (n >= tiles_n) {
+      n -= tiles_n;
+      ++m;
+    }
+  }
+};
+
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_e4m3_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ CUtensorMap tmC, const E4m3Params p) {
@@ -424,7 +451,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint8_t* sW = smem + Cfg::STAGES * Cfg::HALF_BYTES;
   uint8_t* sOut = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
   uint8_t* sSF = sOut + Cfg::STAGING;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + 2 * Cfg::SF_BYTES);
+  float* sBias = reinterpret_cast<float*>(sSF + 2 * Cfg::SF_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + 2 * Cfg::SF_BYTES + Cfg::BIAS_BYTES);
   uint64_t* empty = full + Cfg::STAGES;
   uint64_t* sf_full = empty + Cfg::STAGES;
   uint64_t* sf_empty = sf_full + 2;
@@ -463,25 +491,22 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const uint32_t peer_abort = cluster_addr(tmem_slot + 1, rank ^ 1u);
   grid_dependency_wait();
 
-  const int64_t total = (int64_t)((p.M + 255) / 256) * p.tiles_n;
-  const int64_t first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  TileWalk t((p.M + 255u) / 256u, p.tiles_n, blockIdx.x >> 1, gridDim.x >> 1);
 
   // (loops round the ring of stages, as in the tile kernel, through all tiles)
   if (warp == 0) {
     const uint32_t full_lead = cluster_addr(full, 0);
-    int64_t t = first;
     int kb = 0;
-    int row = (int)(t / p.tiles_n) * 256 + (int)rank * 128;
-    int col = (int)(t % p.tiles_n) * 256 + (int)rank * 128;
-    for (uint32_t ph = 1; t < total; ph ^= 1u) {
+    for (uint32_t ph = 1; t.left; ph ^= 1u) {
 #pragma unroll
       for (int s = 0; s < Cfg::STAGES; ++s) {
-        if (t >= total) break;
+        if (!t.left) break;
         if (!mbar_wait_cluster_warp(&empty[s], ph, abort_flag, p.err)) {
           if (lane == 0) st_cluster_u32(peer_abort, 1);
-          t = total;
+          t.left = 0;
           break;
         }
+        const int row = t.m * 256 + rank * 128, col = t.n * 256 + rank * 128;
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE_BYTES);
           tma_load_2d_pair(&tmA, full_lead + s * 8, sA + s * Cfg::HALF_BYTES, kb * kBlockK, row);
@@ -489,9 +514,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         if (++kb == p.num_kb) {
           kb = 0;
-          t += step;
-          row = (int)(t / p.tiles_n) * 256 + (int)rank * 128;
-          col = (int)(t % p.tiles_n) * 256 + (int)rank * 128;
+          t.next();
         }
       }
     }
@@ -502,12 +525,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const uint64_t dw = sdesc_sw128(smem_u32(sW), 16, 1024);
       const uint64_t dsf = sdesc_rows16(smem_u32(sSF));
       uint32_t u = 0, i = 0;                         // scale words, tiles so far
-      int64_t t = first;
       int kb = 0;
-      for (uint32_t ph = 0; t < total; ph ^= 1u) {
+      for (uint32_t ph = 0; t.left; ph ^= 1u) {
 #pragma unroll
         for (int s = 0; s < Cfg::STAGES; ++s) {
-          if (t >= total) break;
+          if (!t.left) break;
           const uint32_t b = u & 1, sf = tmem + Cfg::SF + b * 12;
           const uint32_t acc = tmem + ((i & 1) ? Cfg::ACC1 : 0u);
           const bool fresh = (kb & 3) == 0;
@@ -519,7 +541,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           ok = ok && mbar_wait_cluster_warp(&full[s], ph, abort_flag, p.err);
           if (!ok) {
             if (lane == 0) st_cluster_u32(peer_abort, 1);
-            t = total;
+            t.left = 0;
             break;
           }
           tc_fence_after();
@@ -545,7 +567,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           ++kb;
           if (last) {
             kb = 0;
-            t += step;
+            t.next();
             ++i;
           }
         }
@@ -556,14 +578,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t sf_full_lead = cluster_addr(sf_full, 0);
     const int groups = (p.num_kb + 3) >> 2;
     uint32_t u = 0;
-    for (int64_t t = first; t < total; t += step) {
-      const int64_t m0 = (t / p.tiles_n) * 256 + rank * 128;
-      const int n0 = (int)(t % p.tiles_n) * 256;
+    for (; t.left; t.next()) {
+      const int m0 = t.m * 256 + rank * 128, n0 = t.n * 256;
       for (int g = 0; g < groups; ++g, ++u) {
         uint32_t a[4], w[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int64_t m = m0 + lane + 32 * j;
+          const int m = m0 + lane + 32 * j;
           a[j] = m < p.M ? __ldg(p.a_scales + (int64_t)g * p.M + m) : 0x7f7f7f7fu;
         }
 #pragma unroll
@@ -593,11 +614,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     uint8_t* box = sOut + (warp - 3) * 4096;
     const uint32_t tempty_lead = cluster_addr(tempty, 0);
     int i = 0;
-    for (int64_t t = first; t < total; t += step, ++i) {
-      const int64_t row0 = (t / p.tiles_n) * 256 + rank * 128 + quarter * 32;
-      const int n0 = (int)(t % p.tiles_n) * 256;
+    for (; t.left; t.next(), ++i) {
+      const int64_t row0 = (int64_t)t.m * 256 + rank * 128 + quarter * 32;
+      const int n0 = t.n * 256;
       const bool overlaps = half != (i & 1);         // this half reads the overlap
       if (!overlaps && lane == 0) mbar_arrive_cluster(tempty_lead);
+      // the tile's bias, 4 columns to a lane, while its MMAs run
+      float* bias = sBias + (warp - 3) * 128;
+      if (p.bias) {
+        const int n = n0 + half * 128 + lane * 4;
+        *reinterpret_cast<float4*>(bias + lane * 4) =
+            n < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + n)) : make_float4(0, 0, 0, 0);
+        __syncwarp();
+      }
       const bool ok = mbar_wait_cluster(&tfull[i & 1], (i >> 1) & 1, abort_flag, p.err);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) st_cluster_u32(peer_abort, 1);
@@ -620,7 +649,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(tempty_lead);
           }
-          finish32(p, v, row0 + lane, n0 + c64 + h * 32, w);
+          finish32(p, v, row0 + lane, n0 + c64 + h * 32, bias + (c64 & 127) + h * 32, w);
           if (hi == 0) {                             // the last store has read the box
             if (lane == 0) bulk_wait_read_all();
             __syncwarp();
