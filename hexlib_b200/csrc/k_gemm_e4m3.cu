@@ -372,47 +372,41 @@ struct PairCfg {
 
 // 32 columns of a row: bias (its 32 values in shared memory), activation, residual, one
 // rounding.
-__device__ __forceinline__ void finish32(const E4m3Params& p, uint32_t (&v)[32], int64_t row,
+__device__ __forceinline__ void finish32(const E4m3Params& p, const uint32_t (&r)[32], int64_t row,
                                          int n, const float* bias, uint32_t (&w)[16]) {
-  const bool row_ok = row < p.M;
+  float2 v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    v[j] = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
   if (p.bias) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 b = *reinterpret_cast<const float4*>(bias + j);
-      v[j] = __float_as_uint(__uint_as_float(v[j]) + b.x);
-      v[j + 1] = __float_as_uint(__uint_as_float(v[j + 1]) + b.y);
-      v[j + 2] = __float_as_uint(__uint_as_float(v[j + 2]) + b.z);
-      v[j + 3] = __float_as_uint(__uint_as_float(v[j + 3]) + b.w);
+    for (int j = 0; j < 16; j += 2) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + 2 * j);
+      v[j] = __fadd2_rn(v[j], make_float2(b.x, b.y));
+      v[j + 1] = __fadd2_rn(v[j + 1], make_float2(b.z, b.w));
     }
   }
   if (p.act == 1) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      const float2 g = gelu_tanh_f2(make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])));
-      v[j] = __float_as_uint(g.x);
-      v[j + 1] = __float_as_uint(g.y);
-    }
+    for (int j = 0; j < 16; ++j) v[j] = gelu_tanh_f2(v[j]);
   } else if (p.act == 2) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(gelu_erf_f(__uint_as_float(v[j])));
+    for (int j = 0; j < 16; ++j) v[j] = make_float2(gelu_erf_f(v[j].x), gelu_erf_f(v[j].y));
   }
-  if (p.resid && row_ok) {
-    const __half* r = p.resid + row * p.N + n;
+  if (p.resid && row < p.M) {
+    const __half* q = p.resid + row * p.N + n;
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      const uint4 u = n + j < p.N ? *reinterpret_cast<const uint4*>(r + j) : make_uint4(0, 0, 0, 0);
+    for (int j = 0; j < 16; j += 4) {
+      const uint4 u = n + 2 * j < p.N ? *reinterpret_cast<const uint4*>(q + 2 * j)
+                                      : make_uint4(0, 0, 0, 0);
       const uint32_t h[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[q]));
-        v[j + 2 * q] = __float_as_uint(__uint_as_float(v[j + 2 * q]) + f.x);
-        v[j + 2 * q + 1] = __float_as_uint(__uint_as_float(v[j + 2 * q + 1]) + f.y);
-      }
+      for (int i = 0; i < 4; ++i)
+        v[j + i] = __fadd2_rn(v[j + i], __half22float2(*reinterpret_cast<const __half2*>(&h[i])));
     }
   }
 #pragma unroll
-  for (int q = 0; q < 16; ++q)
-    w[q] = pack_half2(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
+  for (int j = 0; j < 16; ++j) w[j] = pack_half2(v[j].x, v[j].y);
 }
 
 // The tiles of a CTA pair, `step` apart in row-major order, without a division between
@@ -613,20 +607,24 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int quarter = warp & 3, half = (warp - 3) >> 2;
     uint8_t* box = sOut + (warp - 3) * 4096;
     const uint32_t tempty_lead = cluster_addr(tempty, 0);
+    // a tile's bias, 4 columns to a lane, read while the tile before is finished
+    float* bias = sBias + (warp - 3) * 128;
+    auto bias_of = [&](uint32_t tn) {
+      const int n = tn * 256 + half * 128 + lane * 4;
+      return p.bias && n < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + n))
+                               : make_float4(0, 0, 0, 0);
+    };
+    float4 b4 = bias_of(t.n);
     int i = 0;
-    for (; t.left; t.next(), ++i) {
+    for (; t.left; ++i) {
       const int64_t row0 = (int64_t)t.m * 256 + rank * 128 + quarter * 32;
       const int n0 = t.n * 256;
+      t.next();
       const bool overlaps = half != (i & 1);         // this half reads the overlap
       if (!overlaps && lane == 0) mbar_arrive_cluster(tempty_lead);
-      // the tile's bias, 4 columns to a lane, while its MMAs run
-      float* bias = sBias + (warp - 3) * 128;
-      if (p.bias) {
-        const int n = n0 + half * 128 + lane * 4;
-        *reinterpret_cast<float4*>(bias + lane * 4) =
-            n < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + n)) : make_float4(0, 0, 0, 0);
-        __syncwarp();
-      }
+      *reinterpret_cast<float4*>(bias + lane * 4) = b4;
+      __syncwarp();
+      if (t.left) b4 = bias_of(t.n);
       const bool ok = mbar_wait_cluster(&tfull[i & 1], (i >> 1) & 1, abort_flag, p.err);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) st_cluster_u32(peer_abort, 1);
@@ -651,7 +649,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
           finish32(p, v, row0 + lane, n0 + c64 + h * 32, bias + (c64 & 127) + h * 32, w);
           if (hi == 0) {                             // the last store has read the box
-            if (lane == 0) bulk_wait_read_all();
+            bulk_wait_read_all();                    // (of the lane that issued it)
             __syncwarp();
           }
 #pragma unroll
@@ -661,13 +659,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         fence_proxy_async_shared();
         __syncwarp();
-        if (lane == 0 && row0 < p.M && n0 + c64 < p.N) {
+        if (row0 < p.M && n0 + c64 < p.N && elect_one()) {
           tma_store_3d(&tmC, box, n0 + c64, (int)row0, 0);
           bulk_commit_group();
         }
       }
     }
-    if (lane == 0) bulk_wait_all();
+    bulk_wait_all();
     __syncwarp();
   }
 
