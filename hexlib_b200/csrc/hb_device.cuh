@@ -181,6 +181,14 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t caddr) {
                : "memory");
 }
 
+// The same without ordering the thread's memory writes before it, for a reader that
+// only reports having read: a release waits for the thread's global stores, and a warp
+// that stores rows between its arrivals stood still a thousand cycles at each.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t caddr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(caddr)
+               : "memory");
+}
+
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(

@@ -33,7 +33,8 @@ struct E4m3Params {
   const __half* resid;
   __half* out;
   int M, N, num_kb, act;
-  int tiles_n;                // tiles of 128 features
+  int tiles_n;                // tiles along N
+  int wide;                   // rows of out and resid are whole 16-byte vectors
   int* err;
 };
 
@@ -294,6 +295,8 @@ E4m3Params params_of(const GemmE4m3Desc& g, int* err) {
   p.N = g.N;
   p.num_kb = (int)(e4m3_pitch(g.K) / kBlockK);
   p.act = g.act;
+  p.wide = ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.resid) |
+             static_cast<uintptr_t>(2) * g.N) & 15u) == 0;
   p.err = err;
   return p;
 }
@@ -336,45 +339,50 @@ int launch_tile(const GemmE4m3Desc& g, int split_log2, int* err, cudaStream_t s)
   return HEXLIB_B200_OK;
 }
 
-// ---- CTA pairs, 256 tokens by 256 features ---------------------------------------
+// ---- CTA pairs, 256 tokens by 256 or 192 features ---------------------------------
 //
 // A persistent kernel on clusters of two SMs. Per block of 128 of K each CTA lands its
-// own 128 rows of a and of w (32 KiB), and the leader's MMA thread multiplies the
-// 256 x 256 x 128 block across both SMs: half the fill traffic of one-CTA tiles, which
-// is what bounds an 8-bit mainloop (64 bytes per cycle and SM even so).
+// own half of the rows of a and of w, and the leader's MMA thread multiplies the
+// 256 x BN x 128 block across both SMs: half the fill traffic of one-CTA tiles.
 //
-// Tensor memory holds 512 columns: two 256-column accumulators would leave none for
-// the scales. The accumulators therefore OVERLAP by 24 columns, [0, 256) and
-// [232, 488), and the scales take [488, 512). The epilogue reads the overlap first and
-// tells the MMA thread as soon as it has; the next tile's MMAs start then, while the
-// rest of the tile is finished. That arrival also says that the warp is done with
-// every earlier tile, so one barrier covers both uses.
+// Tensor memory holds 512 columns, 24 of them scales (two buffers). BN = 192 leaves
+// room for two whole accumulators, so a tile's MMAs never wait for the epilogue of the
+// one before; at K = 768 the wait is a third of the time. BN = 256 loads fewer bytes per
+// product, which counts at long K, but its two accumulators OVERLAP by 24 columns,
+// [0, 256) and [232, 488): the epilogue reads the overlap first and says so, and the
+// next tile's MMAs start then, while the rest of the tile is finished.
 //
 //   full[s]     leader: both CTAs' loads of stage s
 //   empty[s]    both: the stage has been read
 //   sf_full[b]  leader: both CTAs have written scale buffer b
 //   sf_empty[b] both: the MMAs that use scale buffer b are done
 //   tfull[a]    both: accumulator a is complete
-//   tempty      leader: the pair's 16 epilogue warps have read the overlap
+//   tempty[a]   leader, BN = 192: the pair's 16 epilogue warps have read accumulator a
+//   tempty[0]   leader, BN = 256: they have read the overlap, and all earlier tiles
+//
+// Epilogue: 8 warps, each 32 rows by BN / 2 columns, 32 columns at a time: from tensor
+// memory through registers and a 2 KiB box in shared memory to rows of 64 bytes. The
+// LSU stores them: it is idle, while 4 KiB TMA stores took turns with the operand loads
+// (16384 x 128 x 2304: 27 us with them).
 constexpr int kPairThreads = 352;   // loads, MMAs, scales, 8 epilogue warps
 
+template <int BN>
 struct PairCfg {
-  static constexpr int STAGES = 5;
-  static constexpr int HALF_BYTES = 128 * kBlockK;
-  static constexpr int STAGE_BYTES = 2 * HALF_BYTES;      // of each CTA
+  static constexpr int STAGES = BN == 256 ? 5 : 6;
+  static constexpr int A_BYTES = 128 * kBlockK;           // of each CTA
+  static constexpr int W_BYTES = BN / 2 * kBlockK;
+  static constexpr int STAGE_BYTES = A_BYTES + W_BYTES;
   static constexpr int SF_BYTES = 512 + 1024;             // own rows of a, all rows of w
-  static constexpr int STAGING = 8 * 4096;                // a 32 x 64 fp16 box per warp
-  static constexpr int BIAS_BYTES = 8 * 512;              // the 128 columns of each
+  static constexpr int BOX_BYTES = 2048;                  // 32 rows of 32 fp16 per warp
+  static constexpr int BIAS_BYTES = BN / 2 * 4;           // the columns of each warp
   static constexpr int SMEM_BYTES =
-      STAGES * STAGE_BYTES + STAGING + 2 * SF_BYTES + BIAS_BYTES + 1024 + 256;
-  static constexpr uint32_t ACC1 = 232, SF = 488;
+      STAGES * STAGE_BYTES + 8 * (BOX_BYTES + BIAS_BYTES) + 2 * SF_BYTES + 1024 + 256;
+  static constexpr uint32_t ACC1 = BN == 256 ? 232 : BN, SF = 488;
 };
 
-// 32 columns of a row: bias (its 32 values in shared memory), activation, residual, one
-// rounding.
-__device__ __forceinline__ void finish32(const E4m3Params& p, const uint32_t (&r)[32], int64_t row,
-                                         int n, const float* bias, uint32_t (&w)[16]) {
-  float2 v[16];
+// 32 columns of a row: bias (its 32 values in shared memory), activation.
+__device__ __forceinline__ void activate32(const E4m3Params& p, const uint32_t (&r)[32],
+                                           const float* bias, float2 (&v)[16]) {
 #pragma unroll
   for (int j = 0; j < 16; ++j)
     v[j] = make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
@@ -393,20 +401,55 @@ __device__ __forceinline__ void finish32(const E4m3Params& p, const uint32_t (&r
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = make_float2(gelu_erf_f(v[j].x), gelu_erf_f(v[j].y));
   }
-  if (p.resid && row < p.M) {
-    const __half* q = p.resid + row * p.N + n;
+}
+
+// A box of 32 rows of 64 bytes, the 16-byte slot q of row r at q ^ (r / 2 % 4): a lane
+// that writes its own row and a quarter warp that reads two rows both touch every bank
+// once.
+__device__ __forceinline__ uint32_t box_at(int r, int q) {
+  return r * 64 + ((q ^ ((r >> 1) & 3)) * 16);
+}
+
+// The box between shared and global memory, rows [row0, row0 + 32) clipped to M and
+// columns [n, n + 32) to N: 16 bytes to a lane where the rows allow it, else 2.
+__device__ __forceinline__ void box_store(const E4m3Params& p, const uint8_t* box, int64_t row0,
+                                          int n, int lane) {
+  if (p.wide) {
 #pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      const uint4 u = n + 2 * j < p.N ? *reinterpret_cast<const uint4*>(q + 2 * j)
-                                      : make_uint4(0, 0, 0, 0);
-      const uint32_t h[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        v[j + i] = __fadd2_rn(v[j + i], __half22float2(*reinterpret_cast<const __half2*>(&h[i])));
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2), q = lane & 3;
+      if (row0 + r < p.M && n + q * 8 < p.N)
+        *reinterpret_cast<uint4*>(p.out + (row0 + r) * p.N + n + q * 8) =
+            *reinterpret_cast<const uint4*>(box + box_at(r, q));
     }
+  } else {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (row0 + r < p.M && n + lane < p.N)
+        p.out[(row0 + r) * p.N + n + lane] =
+            *reinterpret_cast<const __half*>(box + box_at(r, lane >> 3) + (lane & 7) * 2);
   }
+}
+__device__ __forceinline__ void box_load(const E4m3Params& p, uint8_t* box, int64_t row0, int n,
+                                         int lane) {
+  if (p.wide) {
+    uint4 u[4];
 #pragma unroll
-  for (int j = 0; j < 16; ++j) w[j] = pack_half2(v[j].x, v[j].y);
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2), q = lane & 3;
+      u[i] = row0 + r < p.M && n + q * 8 < p.N
+                 ? *reinterpret_cast<const uint4*>(p.resid + (row0 + r) * p.N + n + q * 8)
+                 : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<uint4*>(box + box_at(i * 8 + (lane >> 2), lane & 3)) = u[i];
+  } else {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      *reinterpret_cast<__half*>(box + box_at(r, lane >> 3) + (lane & 7) * 2) =
+          row0 + r < p.M && n + lane < p.N ? p.resid[(row0 + r) * p.N + n + lane] : __half(0.f);
+  }
 }
 
 // The tiles of a CTA pair, `step` apart in row-major order, without a division between
@@ -434,25 +477,26 @@ struct TileWalk {
   }
 };
 
+template <int BN>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_e4m3_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
-                   const __grid_constant__ CUtensorMap tmC, const E4m3Params p) {
-  using Cfg = PairCfg;
+                   const E4m3Params p) {
+  using Cfg = PairCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
-  uint8_t* sW = smem + Cfg::STAGES * Cfg::HALF_BYTES;
-  uint8_t* sOut = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
-  uint8_t* sSF = sOut + Cfg::STAGING;
-  float* sBias = reinterpret_cast<float*>(sSF + 2 * Cfg::SF_BYTES);
-  uint64_t* full = reinterpret_cast<uint64_t*>(sSF + 2 * Cfg::SF_BYTES + Cfg::BIAS_BYTES);
+  uint8_t* sW = smem + Cfg::STAGES * Cfg::A_BYTES;
+  uint8_t* sBox = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
+  uint8_t* sSF = sBox + 8 * Cfg::BOX_BYTES;
+  uint8_t* sBias = sSF + 2 * Cfg::SF_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sBias + 8 * Cfg::BIAS_BYTES);
   uint64_t* empty = full + Cfg::STAGES;
   uint64_t* sf_full = empty + Cfg::STAGES;
   uint64_t* sf_empty = sf_full + 2;
   uint64_t* tfull = sf_empty + 2;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -466,13 +510,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(&sf_full[b], 2);
       mbar_init(&sf_empty[b], 1);
       mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 16);
     }
-    mbar_init(tempty, 16);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmC);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, 512);
@@ -500,11 +543,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           t.left = 0;
           break;
         }
-        const int row = t.m * 256 + rank * 128, col = t.n * 256 + rank * 128;
+        const int row = t.m * 256 + rank * 128, col = t.n * BN + rank * (BN / 2);
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Cfg::STAGE_BYTES);
-          tma_load_2d_pair(&tmA, full_lead + s * 8, sA + s * Cfg::HALF_BYTES, kb * kBlockK, row);
-          tma_load_2d_pair(&tmW, full_lead + s * 8, sW + s * Cfg::HALF_BYTES, kb * kBlockK, col);
+          tma_load_2d_pair(&tmA, full_lead + s * 8, sA + s * Cfg::A_BYTES, kb * kBlockK, row);
+          tma_load_2d_pair(&tmW, full_lead + s * 8, sW + s * Cfg::W_BYTES, kb * kBlockK, col);
         }
         if (++kb == p.num_kb) {
           kb = 0;
@@ -514,7 +557,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      constexpr uint32_t idesc = idesc_e4m3_scaled(256, 256);
+      constexpr uint32_t idesc = idesc_e4m3_scaled(256, BN);
       const uint64_t da = sdesc_sw128(smem_u32(sA), 16, 1024);
       const uint64_t dw = sdesc_sw128(smem_u32(sW), 16, 1024);
       const uint64_t dsf = sdesc_rows16(smem_u32(sSF));
@@ -528,8 +571,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           const uint32_t acc = tmem + ((i & 1) ? Cfg::ACC1 : 0u);
           const bool fresh = (kb & 3) == 0;
           bool ok = true;
-          if (kb == 0 && i > 0)
+          if (kb == 0 && BN == 256 && i > 0)
             ok = mbar_wait_cluster_warp(tempty, (i - 1) & 1, abort_flag, p.err);
+          if (kb == 0 && BN != 256 && i > 1)
+            ok = mbar_wait_cluster_warp(&tempty[i & 1], ((i - 2) >> 1) & 1, abort_flag, p.err);
           if (fresh)
             ok = ok && mbar_wait_cluster_warp(&sf_full[b], (u >> 1) & 1, abort_flag, p.err);
           ok = ok && mbar_wait_cluster_warp(&full[s], ph, abort_flag, p.err);
@@ -550,8 +595,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const uint32_t id = idesc_with_scale_byte(idesc, kb & 3);
 #pragma unroll
             for (int kk = 0; kk < kBlockK / 32; ++kk)
-              umma_e4m3_scaled_pair(acc, da + (s * Cfg::HALF_BYTES + kk * 32 >> 4),
-                                    dw + (s * Cfg::HALF_BYTES + kk * 32 >> 4), id, sf, sf + 4,
+              umma_e4m3_scaled_pair(acc, da + (s * Cfg::A_BYTES + kk * 32 >> 4),
+                                    dw + (s * Cfg::W_BYTES + kk * 32 >> 4), id, sf, sf + 4,
                                     kk > 0 || kb > 0 ? 1u : 0u);
             umma_commit_pair(&empty[s], 0x3);
             if (last_of_word) umma_commit_pair(&sf_empty[b], 0x3);
@@ -573,7 +618,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const int groups = (p.num_kb + 3) >> 2;
     uint32_t u = 0;
     for (; t.left; t.next()) {
-      const int m0 = t.m * 256 + rank * 128, n0 = t.n * 256;
+      const int m0 = t.m * 256 + rank * 128, n0 = t.n * BN;
       for (int g = 0; g < groups; ++g, ++u) {
         uint32_t a[4], w[8];
 #pragma unroll
@@ -601,72 +646,82 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     }
   } else {
-    // Epilogue: TMEM lanes of `quarter`, 128 columns of `half`, 64 at a time, the half's
-    // end that overlaps the other accumulator first (columns 232.. of the first, 0..23
-    // of the second).
+    // Epilogue: TMEM lanes of `quarter`, the columns of `half` (with BN = 256 from the
+    // end that overlaps the other accumulator: columns 232.. of the first, 0..23 of the
+    // second).
+    constexpr int COLS = BN / 2;
     const int quarter = warp & 3, half = (warp - 3) >> 2;
-    uint8_t* box = sOut + (warp - 3) * 4096;
+    uint8_t* box = sBox + (warp - 3) * Cfg::BOX_BYTES;
+    float* bias = reinterpret_cast<float*>(sBias + (warp - 3) * Cfg::BIAS_BYTES);
     const uint32_t tempty_lead = cluster_addr(tempty, 0);
-    // a tile's bias, 4 columns to a lane, read while the tile before is finished
-    float* bias = sBias + (warp - 3) * 128;
-    auto bias_of = [&](uint32_t tn) {
-      const int n = tn * 256 + half * 128 + lane * 4;
-      return p.bias && n < p.N ? __ldg(reinterpret_cast<const float4*>(p.bias + n))
-                               : make_float4(0, 0, 0, 0);
+    // a tile's bias is read while the tile before is finished
+    float next_bias[COLS / 32];
+    auto read_bias = [&](uint32_t tn) {
+#pragma unroll
+      for (int j = 0; j < COLS / 32; ++j) {
+        const int n = tn * BN + half * COLS + j * 32 + lane;
+        next_bias[j] = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
+      }
     };
-    float4 b4 = bias_of(t.n);
-    int i = 0;
+    read_bias(t.n);
+    uint32_t i = 0;
     for (; t.left; ++i) {
       const int64_t row0 = (int64_t)t.m * 256 + rank * 128 + quarter * 32;
-      const int n0 = t.n * 256;
+      const int n0 = t.n * BN + half * COLS;
       t.next();
-      const bool overlaps = half != (i & 1);         // this half reads the overlap
-      if (!overlaps && lane == 0) mbar_arrive_cluster(tempty_lead);
-      *reinterpret_cast<float4*>(bias + lane * 4) = b4;
+      const bool overlaps = BN == 256 && half != (int)(i & 1);   // this half has the overlap
+      if (BN == 256 && !overlaps && lane == 0) mbar_arrive_cluster_relaxed(tempty_lead);
+#pragma unroll
+      for (int j = 0; j < COLS / 32; ++j) bias[j * 32 + lane] = next_bias[j];
       __syncwarp();
-      if (t.left) b4 = bias_of(t.n);
+      if (t.left) read_bias(t.n);
+      if (p.resid) box_load(p, box, row0, n0 + (half ? COLS - 32 : 0), lane);
       const bool ok = mbar_wait_cluster(&tfull[i & 1], (i >> 1) & 1, abort_flag, p.err);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) st_cluster_u32(peer_abort, 1);
         goto out;
       }
       tc_fence_after();
-      const uint32_t tacc =
-          tmem + ((i & 1) ? Cfg::ACC1 : 0u) + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t tacc = tmem + ((i & 1) ? Cfg::ACC1 : 0u) + half * COLS +
+                            ((uint32_t)(quarter * 32) << 16);
 #pragma unroll 1
-      for (int gi = 0; gi < 2; ++gi) {
-        const int c64 = half ? 192 - 64 * gi : 64 * gi;
-#pragma unroll
-        for (int hi = 0; hi < 2; ++hi) {
-          const int h = half ? 1 - hi : hi;
-          uint32_t v[32], w[16];
-          tmem_ld_32x32b_x32(tacc + c64 + h * 32, v);
-          tmem_ld_wait();
-          if (overlaps && gi == 0 && hi == 0) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(tempty_lead);
-          }
-          finish32(p, v, row0 + lane, n0 + c64 + h * 32, bias + (c64 & 127) + h * 32, w);
-          if (hi == 0) {                             // the last store has read the box
-            bulk_wait_read_all();                    // (of the lane that issued it)
-            __syncwarp();
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(box + lane * 128 + (((h * 4 + j) ^ (lane & 7)) * 16)) =
-                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      for (int j = 0; j < COLS / 32; ++j) {
+        const int c = half ? COLS - 32 - 32 * j : 32 * j;
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tacc + c, r);
+        tmem_ld_wait();
+        if (BN == 256 ? overlaps && j == 0 : j == COLS / 32 - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster_relaxed(tempty_lead + (BN == 256 ? 0 : (i & 1) * 8));
         }
-        fence_proxy_async_shared();
+        float2 v[16];
+        activate32(p, r, bias + c, v);
+        if (p.resid) {
+          if (j > 0) box_load(p, box, row0, n0 + c, lane);
+          __syncwarp();
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint4* slot = reinterpret_cast<uint4*>(box + box_at(lane, q));
+          if (p.resid) {
+            const uint4 u = *slot;
+            const uint32_t h[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[4 * q + e] = __fadd2_rn(v[4 * q + e],
+                                        __half22float2(*reinterpret_cast<const __half2*>(&h[e])));
+          }
+          *slot = make_uint4(pack_half2(v[4 * q].x, v[4 * q].y),
+                             pack_half2(v[4 * q + 1].x, v[4 * q + 1].y),
+                             pack_half2(v[4 * q + 2].x, v[4 * q + 2].y),
+                             pack_half2(v[4 * q + 3].x, v[4 * q + 3].y));
+        }
         __syncwarp();
-        if (row0 < p.M && n0 + c64 < p.N && elect_one()) {
-          tma_store_3d(&tmC, box, n0 + c64, (int)row0, 0);
-          bulk_commit_group();
-        }
+        box_store(p, box, row0, n0 + c, lane);
+        __syncwarp();                                // read before the next chunk's writes
       }
     }
-    bulk_wait_all();
-    __syncwarp();
   }
 
 out:
@@ -679,41 +734,56 @@ out:
   }
 }
 
+template <int BN>
 std::atomic<int> g_pairs{0};   // pairs resident at once, 0 until the kernel is loaded
 
+template <int BN>
 int launch_pair(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
+  using Cfg = PairCfg<BN>;
   const uint64_t pitch = (uint64_t)e4m3_pitch(g.K);
-  CUtensorMap ta, tw, tc;
+  CUtensorMap ta, tw;
   if (!make_tmap_2d_u8(&ta, g.a, pitch, (uint64_t)g.M, 128) ||
-      !make_tmap_2d_u8(&tw, g.w, pitch, (uint64_t)g.N, 128) ||
-      !make_tmap_3d_f16(&tc, g.out, (uint64_t)g.N, (uint64_t)g.M, 1, 64, 32))
+      !make_tmap_2d_u8(&tw, g.w, pitch, (uint64_t)g.N, BN / 2))
     return HEXLIB_B200_ERR_CUDA;
   E4m3Params p = params_of(g, err);
-  p.tiles_n = (g.N + 255) / 256;
+  p.tiles_n = (g.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)((g.M + 255) / 256) * p.tiles_n;
-  const int64_t pairs = g_pairs.load(std::memory_order_relaxed);
+  if (tiles > 0x3fffffff) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  const int64_t pairs = g_pairs<BN>.load(std::memory_order_relaxed);
+  if (pairs <= 0) return HEXLIB_B200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)), 1, 1);
   cfg.blockDim = dim3(kPairThreads, 1, 1);
-  cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
+  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   cfg.attrs = cluster_of(attr, 2);
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, gemm_e4m3_pair, ta, tw, tc, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, gemm_e4m3_pair<BN>, ta, tw, p) != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
   return HEXLIB_B200_OK;
 }
 
-// What the pair kernel asks of the output: whole 16-byte vectors in every row.
-bool pair_can(const GemmE4m3Desc& g) {
-  const uintptr_t bits = reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.resid) |
-                         reinterpret_cast<uintptr_t>(g.bias) | static_cast<uintptr_t>(2) * g.N;
-  return bits % 16 == 0 && g_pairs.load(std::memory_order_relaxed) > 0;
+template <int BN>
+bool load_pair() {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(512, 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = PairCfg<BN>::SMEM_BYTES;
+  cudaLaunchAttribute attr[1];
+  cfg.attrs = cluster_of(attr, 2);
+  cfg.numAttrs = 1;
+  int pairs = 0;
+  if (cudaFuncSetAttribute(gemm_e4m3_pair<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           PairCfg<BN>::SMEM_BYTES) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&pairs, gemm_e4m3_pair<BN>, &cfg) != cudaSuccess)
+    return false;
+  g_pairs<BN>.store(pairs, std::memory_order_relaxed);
+  return pairs > 0;
 }
 
 }  // namespace
@@ -727,30 +797,16 @@ int gemm_e4m3_kernels_init() {
                            TileCfg<64>::smem(2)) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_e4m3_tile<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            TileCfg<128>::smem(2)) != cudaSuccess ||
-      cudaFuncSetAttribute(gemm_e4m3_pair, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           PairCfg::SMEM_BYTES) != cudaSuccess) {
+      !load_pair<256>() || !load_pair<192>()) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(512, 1, 1);
-  cfg.blockDim = dim3(kPairThreads, 1, 1);
-  cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
-  cudaLaunchAttribute attr[1];
-  cfg.attrs = cluster_of(attr, 2);
-  cfg.numAttrs = 1;
-  int pairs = 0;
-  if (cudaOccupancyMaxActiveClusters(&pairs, gemm_e4m3_pair, &cfg) != cudaSuccess) {
-    cudaGetLastError();
-    return HEXLIB_B200_ERR_CUDA;
-  }
-  g_pairs.store(pairs, std::memory_order_relaxed);
   return HEXLIB_B200_OK;
 }
 
 int launch_gemm_e4m3(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
-  if (g.M > 256 && (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) >= 37 && pair_can(g))
-    return launch_pair(g, err, s);
+  if (g.M > 256 && (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) >= 37)
+    return g.K > 1024 ? launch_pair<256>(g, err, s) : launch_pair<192>(g, err, s);
   const int num_kb = (int)(e4m3_pitch(g.K) / kBlockK);
   const int bn = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
   const int64_t tiles = (int64_t)((g.N + 127) / 128) * ((g.M + bn - 1) / bn);

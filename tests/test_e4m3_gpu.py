@@ -248,7 +248,9 @@ def test_empty_batches_launch_nothing():
 @pytest.mark.parametrize("M,K,N,act,with_bias,with_resid", [
     (2500, 513, 1000, 0, False, False), (4097, 1100, 1032, 0, True, True), (9000, 300, 1288, 1, True, False),
     (9473, 640, 520, 1, False, True), (5000, 128, 2048, 0, True, False), (3000, 2100, 1536, 2, True, True),
-    (19000, 1, 264, 0, False, False), (20000, 260, 512, 0, False, False)])
+    (19000, 1, 264, 0, False, False), (20000, 260, 512, 0, False, False),
+    (2600, 1500, 1001, 0, True, True), (2600, 1500, 1002, 1, True, False), (9500, 300, 777, 0, False, True),
+    (9500, 300, 770, 2, True, True), (2304, 8200, 1280, 0, True, False)])
 def test_product_of_many_tiles(M, K, N, act, with_bias, with_resid):
     rng = np.random.default_rng(M + K)
     a, w = operands(rng, M, K, N, spread=3)
