@@ -13,6 +13,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <math.h>
+
 #include <atomic>
 
 #include "hb_device.cuh"
@@ -67,7 +69,7 @@ struct TileCfg {
   static constexpr int STAGES = 4;
   static constexpr int SF_BYTES = 2 * 2 * 512;                    // two buffers of w and a
   static constexpr int PART_BYTES = BN * 128 * 4;                 // sums from the other ranks
-  static constexpr int TMEM_COLS = BN == 16 ? 32 : 2 * BN;        // accumulator + 16 of scales
+  static constexpr int TMEM_COLS = 2 * BN;                        // accumulator + 16 of scales
   static constexpr int smem(int split) {
     return STAGES * STAGE_BYTES + SF_BYTES + (split > 1 ? PART_BYTES : 0) + 1024 + 256;
   }
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tmem_ld_wait();
     if (split > 1) {
       // token c goes to rank c / cols, at [this rank][c % cols][feature] there
-      constexpr int BN_LOG2 = BN == 16 ? 4 : BN == 32 ? 5 : BN == 64 ? 6 : 7;
+      constexpr int BN_LOG2 = BN == 16 ? 4 : BN == 32 ? 5 : 6;
       const int cols_log2 = BN_LOG2 - split_log2, cols = 1 << cols_log2;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
@@ -339,36 +341,40 @@ int launch_tile(const GemmE4m3Desc& g, int split_log2, int* err, cudaStream_t s)
   return HEXLIB_B200_OK;
 }
 
-// ---- CTA pairs, 256 tokens by 256 or 192 features ---------------------------------
+// ---- CTA pairs, 256 tokens by 256 features ---------------------------------------
 //
 // A persistent kernel on clusters of two SMs. Per block of 128 of K each CTA lands its
-// own half of the rows of a and of w, and the leader's MMA thread multiplies the
-// 256 x BN x 128 block across both SMs: half the fill traffic of one-CTA tiles.
+// own 128 rows of a and of w (32 KiB), and the leader's MMA thread multiplies the
+// 256 x 256 x 128 block across both SMs: half the fill traffic of one-CTA tiles. What
+// bounds the mainloop is shared memory: at the tensor cores' full rate (512 cycles a
+// block) reading the operands and landing the next ones takes all of its 128 bytes a
+// cycle. Measured, the four MMAs of a block take 528 cycles with a quarter of the loads
+// beside them, 571 with half, about 640 with all.
 //
-// Tensor memory holds 512 columns, 24 of them scales (two buffers). BN = 192 leaves
-// room for two whole accumulators, so a tile's MMAs never wait for the epilogue of the
-// one before; at K = 768 the wait is a third of the time. BN = 256 loads fewer bytes per
-// product, which counts at long K, but its two accumulators OVERLAP by 24 columns,
-// [0, 256) and [232, 488): the epilogue reads the overlap first and says so, and the
-// next tile's MMAs start then, while the rest of the tile is finished.
+// Tensor memory holds 512 columns: two 256-column accumulators would leave none for
+// the scales. The accumulators therefore OVERLAP by 24 columns, [0, 256) and
+// [232, 488), and the scales take [488, 512). The epilogue reads the overlap first and
+// tells the MMA thread as soon as it has; the next tile's MMAs start then, while the
+// rest of the tile is finished. That arrival also says that the warp is done with
+// every earlier tile, so one barrier covers both uses. (Tiles of 192 columns with two
+// whole accumulators: 16384 x 768 x 2304 in 42.5 us against 37.6, 8192 x 4096 x 4096 in
+// 134 against 108; narrower MMAs re-read the tokens' rows more often.)
 //
 //   full[s]     leader: both CTAs' loads of stage s
 //   empty[s]    both: the stage has been read
 //   sf_full[b]  leader: both CTAs have written scale buffer b
 //   sf_empty[b] both: the MMAs that use scale buffer b are done
 //   tfull[a]    both: accumulator a is complete
-//   tempty[a]   leader, BN = 192: the pair's 16 epilogue warps have read accumulator a
-//   tempty[0]   leader, BN = 256: they have read the overlap, and all earlier tiles
+//   tempty      leader: the pair's 16 epilogue warps have read the overlap
 //
-// Epilogue: 8 warps, each 32 rows by BN / 2 columns, 32 columns at a time: from tensor
-// memory through registers and a 2 KiB box in shared memory to rows of 64 bytes. The
-// LSU stores them: it is idle, while 4 KiB TMA stores took turns with the operand loads
-// (16384 x 128 x 2304: 27 us with them).
+// Epilogue: 8 warps, each 32 rows by 128 columns, 32 columns at a time: from tensor
+// memory through registers and a 2 KiB box in shared memory to rows of 64 bytes, stored
+// by the LSU at any alignment.
 constexpr int kPairThreads = 352;   // loads, MMAs, scales, 8 epilogue warps
 
-template <int BN>
 struct PairCfg {
-  static constexpr int STAGES = BN == 256 ? 5 : 6;
+  static constexpr int BN = 256;
+  static constexpr int STAGES = 5;
   static constexpr int A_BYTES = 128 * kBlockK;           // of each CTA
   static constexpr int W_BYTES = BN / 2 * kBlockK;
   static constexpr int STAGE_BYTES = A_BYTES + W_BYTES;
@@ -377,7 +383,7 @@ struct PairCfg {
   static constexpr int BIAS_BYTES = BN / 2 * 4;           // the columns of each warp
   static constexpr int SMEM_BYTES =
       STAGES * STAGE_BYTES + 8 * (BOX_BYTES + BIAS_BYTES) + 2 * SF_BYTES + 1024 + 256;
-  static constexpr uint32_t ACC1 = BN == 256 ? 232 : BN, SF = 488;
+  static constexpr uint32_t ACC1 = 232, SF = 488;
 };
 
 // 32 columns of a row: bias (its 32 values in shared memory), activation.
@@ -477,11 +483,11 @@ struct TileWalk {
   }
 };
 
-template <int BN>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_e4m3_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                    const E4m3Params p) {
-  using Cfg = PairCfg<BN>;
+  using Cfg = PairCfg;
+  constexpr int BN = Cfg::BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -496,7 +502,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint64_t* sf_empty = sf_full + 2;
   uint64_t* tfull = sf_empty + 2;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -510,8 +516,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(&sf_full[b], 2);
       mbar_init(&sf_empty[b], 1);
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 16);
     }
+    mbar_init(tempty, 16);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
@@ -571,10 +577,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           const uint32_t acc = tmem + ((i & 1) ? Cfg::ACC1 : 0u);
           const bool fresh = (kb & 3) == 0;
           bool ok = true;
-          if (kb == 0 && BN == 256 && i > 0)
+          if (kb == 0 && i > 0)
             ok = mbar_wait_cluster_warp(tempty, (i - 1) & 1, abort_flag, p.err);
-          if (kb == 0 && BN != 256 && i > 1)
-            ok = mbar_wait_cluster_warp(&tempty[i & 1], ((i - 2) >> 1) & 1, abort_flag, p.err);
           if (fresh)
             ok = ok && mbar_wait_cluster_warp(&sf_full[b], (u >> 1) & 1, abort_flag, p.err);
           ok = ok && mbar_wait_cluster_warp(&full[s], ph, abort_flag, p.err);
@@ -646,9 +650,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     }
   } else {
-    // Epilogue: TMEM lanes of `quarter`, the columns of `half` (with BN = 256 from the
-    // end that overlaps the other accumulator: columns 232.. of the first, 0..23 of the
-    // second).
+    // Epilogue: TMEM lanes of `quarter`, the columns of `half` from the end that may
+    // overlap the other accumulator (columns 232.. of the first, 0..23 of the second).
     constexpr int COLS = BN / 2;
     const int quarter = warp & 3, half = (warp - 3) >> 2;
     uint8_t* box = sBox + (warp - 3) * Cfg::BOX_BYTES;
@@ -669,8 +672,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int64_t row0 = (int64_t)t.m * 256 + rank * 128 + quarter * 32;
       const int n0 = t.n * BN + half * COLS;
       t.next();
-      const bool overlaps = BN == 256 && half != (int)(i & 1);   // this half has the overlap
-      if (BN == 256 && !overlaps && lane == 0) mbar_arrive_cluster_relaxed(tempty_lead);
+      const bool overlaps = half != (int)(i & 1);    // this half has the overlap
+      if (!overlaps && lane == 0) mbar_arrive_cluster_relaxed(tempty_lead);
 #pragma unroll
       for (int j = 0; j < COLS / 32; ++j) bias[j * 32 + lane] = next_bias[j];
       __syncwarp();
@@ -690,10 +693,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         uint32_t r[32];
         tmem_ld_32x32b_x32(tacc + c, r);
         tmem_ld_wait();
-        if (BN == 256 ? overlaps && j == 0 : j == COLS / 32 - 1) {
+        if (overlaps && j == 0) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(tempty_lead + (BN == 256 ? 0 : (i & 1) * 8));
+          if (lane == 0) mbar_arrive_cluster_relaxed(tempty_lead);
         }
         float2 v[16];
         activate32(p, r, bias + c, v);
@@ -734,12 +737,11 @@ out:
   }
 }
 
-template <int BN>
 std::atomic<int> g_pairs{0};   // pairs resident at once, 0 until the kernel is loaded
 
-template <int BN>
 int launch_pair(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
-  using Cfg = PairCfg<BN>;
+  using Cfg = PairCfg;
+  constexpr int BN = Cfg::BN;
   const uint64_t pitch = (uint64_t)e4m3_pitch(g.K);
   CUtensorMap ta, tw;
   if (!make_tmap_2d_u8(&ta, g.a, pitch, (uint64_t)g.M, 128) ||
@@ -749,7 +751,7 @@ int launch_pair(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
   p.tiles_n = (g.N + BN - 1) / BN;
   const int64_t tiles = (int64_t)((g.M + 255) / 256) * p.tiles_n;
   if (tiles > 0x3fffffff) return HEXLIB_B200_ERR_INVAL_PARAMS;
-  const int64_t pairs = g_pairs<BN>.load(std::memory_order_relaxed);
+  const int64_t pairs = g_pairs.load(std::memory_order_relaxed);
   if (pairs <= 0) return HEXLIB_B200_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs)), 1, 1);
@@ -761,28 +763,27 @@ int launch_pair(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, gemm_e4m3_pair<BN>, ta, tw, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, gemm_e4m3_pair, ta, tw, p) != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
   return HEXLIB_B200_OK;
 }
 
-template <int BN>
 bool load_pair() {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(512, 1, 1);
   cfg.blockDim = dim3(kPairThreads, 1, 1);
-  cfg.dynamicSmemBytes = PairCfg<BN>::SMEM_BYTES;
+  cfg.dynamicSmemBytes = PairCfg::SMEM_BYTES;
   cudaLaunchAttribute attr[1];
   cfg.attrs = cluster_of(attr, 2);
   cfg.numAttrs = 1;
   int pairs = 0;
-  if (cudaFuncSetAttribute(gemm_e4m3_pair<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           PairCfg<BN>::SMEM_BYTES) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&pairs, gemm_e4m3_pair<BN>, &cfg) != cudaSuccess)
+  if (cudaFuncSetAttribute(gemm_e4m3_pair, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           PairCfg::SMEM_BYTES) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&pairs, gemm_e4m3_pair, &cfg) != cudaSuccess)
     return false;
-  g_pairs<BN>.store(pairs, std::memory_order_relaxed);
+  g_pairs.store(pairs, std::memory_order_relaxed);
   return pairs > 0;
 }
 
@@ -795,29 +796,59 @@ int gemm_e4m3_kernels_init() {
                            TileCfg<32>::smem(2)) != cudaSuccess ||
       cudaFuncSetAttribute(gemm_e4m3_tile<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            TileCfg<64>::smem(2)) != cudaSuccess ||
-      cudaFuncSetAttribute(gemm_e4m3_tile<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           TileCfg<128>::smem(2)) != cudaSuccess ||
-      !load_pair<256>() || !load_pair<192>()) {
+      !load_pair()) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
   return HEXLIB_B200_OK;
 }
 
-int launch_gemm_e4m3(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
-  if (g.M > 256 && (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) >= 37)
-    return g.K > 1024 ? launch_pair<256>(g, err, s) : launch_pair<192>(g, err, s);
-  const int num_kb = (int)(e4m3_pitch(g.K) / kBlockK);
-  const int bn = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
-  const int64_t tiles = (int64_t)((g.N + 127) / 128) * ((g.M + bn - 1) / bn);
-  int split = 0;
-  while (split < 3 && (tiles << (split + 1)) <= 296 && num_kb >= 4 << split) ++split;
-  switch (bn) {
-    case 16: return launch_tile<16>(g, split, err, s);
-    case 32: return launch_tile<32>(g, split, err, s);
-    case 64: return launch_tile<64>(g, split, err, s);
+// The kernel and tiling with the least estimated time, in us. The estimate is a fixed
+// cost, the blocks of K a CTA goes through at the rate measured for one or two CTAs on an
+// SM (68 and 108 bytes a ns), its epilogue, and the joining of a split; w from memory at
+// 6 TB/s bounds the loop below. It was fitted to sweeps of every choice: 4096 x 4096 for 1 token 8.5 us on
+// 16-token tiles split by 4 (16.9 unsplit), for 256 tokens 16.0 on 64-token tiles (22.0 on
+// pairs, 27 split); 1000 x 1000 for 2000 tokens 10.2 on pairs and on 64-token tiles,
+// 2304 x 256 for 4096 tokens 11.4 on pairs.
+struct Choice {
+  int bn, split_log2;                      // bn = 0: CTA pairs
+};
+
+Choice choose(const GemmE4m3Desc& g) {
+  const double kb = (double)(e4m3_pitch(g.K) / kBlockK);
+  const int64_t pair_tiles = (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256);
+  const double from_memory = kb * kBlockK * g.N / 6000e3;
+  Choice best = {0, 0};
+  double least = 5.0 + (double)((pair_tiles + 73) / 74) * (1.8 + 0.43 * kb);
+  for (int bn = 16; bn <= 64; bn *= 2) {
+    const int64_t tiles = (int64_t)((g.N + 127) / 128) * ((g.M + bn - 1) / bn);
+    for (int sl = 0; sl <= 3 && kb >= (2 << sl) - (sl == 0); ++sl) {
+      const int64_t ctas = tiles << sl, resident = bn == 64 && sl > 0 ? 1 : 2;
+      if (sl > 0 && ctas > 148 * resident) break;
+      const int64_t waves = (ctas + 148 * resident - 1) / (148 * resident);
+      const int64_t beside = ctas > 148 ? resident : 1;      // CTAs on an SM at once
+      const double bytes = (double)(128 + bn) * kBlockK * beside;
+      double loop = (double)waves * ceil(kb / (1 << sl)) * bytes / (beside == 1 ? 68e3 : 108e3);
+      if (loop < from_memory) loop = from_memory;
+      const double finish = (double)waves * beside * 0.02 * bn;
+      const double t = 4.0 + loop + finish + (sl ? 0.5 + 0.036 * bn : 0.0);
+      if (t < least) {
+        least = t;
+        best = {bn, sl};
+      }
+    }
   }
-  return launch_tile<128>(g, split, err, s);
+  return best;
+}
+
+int launch_gemm_e4m3(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
+  const Choice c = choose(g);
+  switch (c.bn) {
+    case 16: return launch_tile<16>(g, c.split_log2, err, s);
+    case 32: return launch_tile<32>(g, c.split_log2, err, s);
+    case 64: return launch_tile<64>(g, c.split_log2, err, s);
+  }
+  return launch_pair(g, err, s);
 }
 
 }  // namespace hb
