@@ -21,28 +21,28 @@ struct RopeShape {
   int tokens;      // of a CTA
   int pairs;       // rot / 2
   int rot_items;   // items of a head that rotate, then those that are copied
-  int items;       // of a head
+  int items;       // of a head, of them the ones to do (in place nothing is copied)
   int head_split;  // CTAs that share a token tile's heads
   int heads;       // of a CTA
+  // 2^32 / items and 2^32 / heads, rounded up: for more than one, i / items is the high
+  // word of the product for every i with i * items < 2^32
+  uint32_t per_item, per_head;
 };
 
-// The phases of a tile of tokens are turned into cosines and sines once, in shared
-// memory, for all heads; then a thread takes an item of 16 (half layout: 8 pairs) or 8
-// (interleaved: 4 pairs) elements of a head at a time, in 16-byte loads and stores.
-// An item's cosines lie `stride` apart, so that the threads of a warp, which take
-// consecutive items, read consecutive words.
-//
-// VEC: D and the row strides whole 16-byte vectors, rot whole items. Otherwise an item
-// is one pair, or one element copied.
-template <bool VEC, bool INTERLEAVED>
-__global__ void __launch_bounds__(kThreads) rope_pos_tile(const RopePosDesc d, const RopeShape sh) {
-  extern __shared__ float2 cs[];                       // [tokens][pairs]
-  constexpr int PAIRS = VEC ? (INTERLEAVED ? 4 : 8) : 1;
-  const int tile = blockIdx.x / sh.head_split;
-  const int h0 = (blockIdx.x % sh.head_split) * sh.heads;
-  const int heads = min(sh.heads, d.H - h0);
-  const int64_t t0 = (int64_t)tile * sh.tokens;
-  const int tokens = (int)min((int64_t)sh.tokens, d.T - t0);
+__device__ __forceinline__ float2 halves(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The cosine and sine of every pair of a tile of tokens, for all its heads, pair j at
+// (j % P) * n + j / P: the P pairs of an item n apart, so that the threads of a warp,
+// which take consecutive items, read consecutive words.
+template <int P>
+__device__ __forceinline__ void tile_phases(const RopePosDesc& d, const RopeShape& sh, int64_t t0,
+                                            int tokens, float2* cs) {
   for (int i = threadIdx.x; i < tokens * sh.pairs; i += kThreads) {
     const int t = i / sh.pairs, j = i - t * sh.pairs;
     const int ax = d.axis ? min(max(__ldg(d.axis + j), 0), d.n_axes - 1) : 0;
@@ -50,59 +50,121 @@ __global__ void __launch_bounds__(kThreads) rope_pos_tile(const RopePosDesc d, c
     const uint64_t phase = (uint64_t)pos * __ldg((const unsigned long long*)d.table + j);
     float s, c;
     sincospif((float)(int32_t)(phase >> 32) * 0x1p-31f, &s, &c);
-    cs[t * sh.pairs + (j % PAIRS) * sh.rot_items + j / PAIRS] =
-        make_float2(d.mscale * c, d.mscale * s);
+    cs[t * sh.pairs + (j % P) * sh.rot_items + j / P] = make_float2(d.mscale * c, d.mscale * s);
   }
-  __syncthreads();
-  const bool in_place = d.x == d.y;
-  const int per_head = in_place ? sh.rot_items : sh.items;
+}
+
+// Rows of whole 16-byte vectors: an item is 16 elements of a head (half layout, 8 pairs)
+// or 8 (interleaved, 4 pairs; or copied). Bound by memory; a thread has two items in
+// flight, the first two from before the phases are formed, which hides the positions'
+// way through memory behind the rows' (32768 tokens of 40 of 48 heads of 128: 112 us,
+// 5.97 TB/s; 135 without, 118 with four items in flight and half the warps; 4097 tokens
+// of 24 heads of 64, three axes: 8.0 us, of which 3.8 are memory's).
+constexpr int kBatch = 2;
+
+template <bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rope_pos_vec(const RopePosDesc d, const RopeShape sh) {
+  extern __shared__ float2 cs[];                       // [tokens][pairs]
+  constexpr int VECS = INTERLEAVED ? 1 : 2;            // of a rotating item
+  const int tile = blockIdx.x / sh.head_split;
+  const int h0 = (blockIdx.x % sh.head_split) * sh.heads;
+  const int heads = min(sh.heads, d.H - h0);
+  const int64_t t0 = (int64_t)tile * sh.tokens;
+  const int tokens = (int)min((int64_t)sh.tokens, d.T - t0);
+  // (the last CTA of a split may have fewer heads; items past them are skipped)
+  const uint32_t total = tokens * sh.heads * sh.items;
   const int half = d.rot >> 1;
-  const int total = tokens * heads * per_head;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int th = i / per_head, item = i - th * per_head;
-    const int t = th / heads, h = h0 + th - t * heads;
+  struct Item {
+    int t, h, item;                                    // h < 0: none
+  };
+  auto item_of = [&](uint32_t i) {
+    const uint32_t th = sh.items == 1 ? i : __umulhi(i, sh.per_item);
+    const uint32_t t = sh.heads == 1 ? th : __umulhi(th, sh.per_head);
+    const int h = th - t * sh.heads;
+    return Item{(int)t, i < total && h < heads ? h : -1, (int)(i - th * sh.items)};
+  };
+  auto first_of = [&](const Item& m) {                 // its first element within the head
+    return m.item < sh.rot_items ? m.item * 8 : d.rot + (m.item - sh.rot_items) * 8;
+  };
+  uint4 u[kBatch][VECS];
+  auto load = [&](uint32_t i0) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const Item m = item_of(i0 + b * kThreads);
+      if (m.h < 0) continue;
+      const __half* x = (const __half*)d.x + (t0 + m.t) * d.x_stride + (int64_t)(h0 + m.h) * d.D +
+                        first_of(m);
+      u[b][0] = *reinterpret_cast<const uint4*>(x);
+      if (!INTERLEAVED && m.item < sh.rot_items)
+        u[b][VECS - 1] = *reinterpret_cast<const uint4*>(x + half);
+    }
+  };
+  load(threadIdx.x);
+  tile_phases<INTERLEAVED ? 4 : 8>(d, sh, t0, tokens, cs);
+  __syncthreads();
+  for (uint32_t i0 = threadIdx.x; i0 < total; i0 += kBatch * kThreads) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const Item m = item_of(i0 + b * kThreads);
+      if (m.h < 0) continue;
+      __half* y = (__half*)d.y + (t0 + m.t) * d.y_stride + (int64_t)(h0 + m.h) * d.D + first_of(m);
+      if (m.item < sh.rot_items) {
+        const float2* c = cs + m.t * sh.pairs + m.item;
+        uint32_t a[4] = {u[b][0].x, u[b][0].y, u[b][0].z, u[b][0].w};
+        if constexpr (INTERLEAVED) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 f = halves(a[q]), k = c[q * sh.rot_items];
+            a[q] = pack(f.x * k.x - f.y * k.y, f.x * k.y + f.y * k.x);
+          }
+        } else {
+          uint32_t e[4] = {u[b][VECS - 1].x, u[b][VECS - 1].y, u[b][VECS - 1].z, u[b][VECS - 1].w};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float2 fa = halves(a[q]), fb = halves(e[q]);
+            const float2 k0 = c[2 * q * sh.rot_items], k1 = c[(2 * q + 1) * sh.rot_items];
+            a[q] = pack(fa.x * k0.x - fb.x * k0.y, fa.y * k1.x - fb.y * k1.y);
+            e[q] = pack(fa.x * k0.y + fb.x * k0.x, fa.y * k1.y + fb.y * k1.x);
+          }
+          *reinterpret_cast<uint4*>(y + half) = make_uint4(e[0], e[1], e[2], e[3]);
+        }
+        u[b][0] = make_uint4(a[0], a[1], a[2], a[3]);
+      }
+      *reinterpret_cast<uint4*>(y) = u[b][0];
+    }
+    load(i0 + kBatch * kThreads);
+  }
+}
+
+// Any rows: an item is one pair, or one element copied.
+template <bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rope_pos_any(const RopePosDesc d, const RopeShape sh) {
+  extern __shared__ float2 cs[];
+  const int tile = blockIdx.x / sh.head_split;
+  const int h0 = (blockIdx.x % sh.head_split) * sh.heads;
+  const int heads = min(sh.heads, d.H - h0);
+  const int64_t t0 = (int64_t)tile * sh.tokens;
+  const int tokens = (int)min((int64_t)sh.tokens, d.T - t0);
+  tile_phases<1>(d, sh, t0, tokens, cs);
+  __syncthreads();
+  const int half = d.rot >> 1;
+  const int64_t total = (int64_t)tokens * heads * sh.items;
+  for (int64_t i = threadIdx.x; i < total; i += kThreads) {
+    const int64_t th = i / sh.items;
+    const int item = (int)(i - th * sh.items);
+    const int t = (int)(th / heads), h = h0 + (int)(th - (int64_t)t * heads);
     const __half* x = (const __half*)d.x + (t0 + t) * d.x_stride + (int64_t)h * d.D;
     __half* y = (__half*)d.y + (t0 + t) * d.y_stride + (int64_t)h * d.D;
     if (item >= sh.rot_items) {
-      const int e = d.rot + (item - sh.rot_items) * (VEC ? 8 : 1);
-      if constexpr (VEC) *reinterpret_cast<uint4*>(y + e) = *reinterpret_cast<const uint4*>(x + e);
-      else y[e] = x[e];
+      const int e = d.rot + item - sh.rot_items;
+      y[e] = x[e];
       continue;
     }
-    const float2* c = cs + t * sh.pairs + item;
-    if constexpr (!VEC) {
-      const int ia = INTERLEAVED ? 2 * item : item, ib = INTERLEAVED ? ia + 1 : ia + half;
-      const float a = __half2float(x[ia]), b = __half2float(x[ib]);
-      y[ia] = __float2half_rn(a * c->x - b * c->y);
-      y[ib] = __float2half_rn(a * c->y + b * c->x);
-    } else if constexpr (INTERLEAVED) {
-      const uint4 u = *reinterpret_cast<const uint4*>(x + item * 8);
-      uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
-        const float2 k = c[q * sh.rot_items];
-        const __half2 r = __floats2half2_rn(f.x * k.x - f.y * k.y, f.x * k.y + f.y * k.x);
-        w[q] = *reinterpret_cast<const uint32_t*>(&r);
-      }
-      *reinterpret_cast<uint4*>(y + item * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
-      const uint4 ua = *reinterpret_cast<const uint4*>(x + item * 8);
-      const uint4 ub = *reinterpret_cast<const uint4*>(x + half + item * 8);
-      uint32_t a[4] = {ua.x, ua.y, ua.z, ua.w}, b[4] = {ub.x, ub.y, ub.z, ub.w};
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float2 fa = __half22float2(*reinterpret_cast<const __half2*>(&a[q]));
-        const float2 fb = __half22float2(*reinterpret_cast<const __half2*>(&b[q]));
-        const float2 k0 = c[2 * q * sh.rot_items], k1 = c[(2 * q + 1) * sh.rot_items];
-        const __half2 ra = __floats2half2_rn(fa.x * k0.x - fb.x * k0.y, fa.y * k1.x - fb.y * k1.y);
-        const __half2 rb = __floats2half2_rn(fa.x * k0.y + fb.x * k0.x, fa.y * k1.y + fb.y * k1.x);
-        a[q] = *reinterpret_cast<const uint32_t*>(&ra);
-        b[q] = *reinterpret_cast<const uint32_t*>(&rb);
-      }
-      *reinterpret_cast<uint4*>(y + item * 8) = make_uint4(a[0], a[1], a[2], a[3]);
-      *reinterpret_cast<uint4*>(y + half + item * 8) = make_uint4(b[0], b[1], b[2], b[3]);
-    }
+    const float2 c = cs[t * sh.pairs + item];
+    const int ia = INTERLEAVED ? 2 * item : item, ib = INTERLEAVED ? ia + 1 : ia + half;
+    const float a = __half2float(x[ia]), b = __half2float(x[ib]);
+    y[ia] = __float2half_rn(a * c.x - b * c.y);
+    y[ib] = __float2half_rn(a * c.y + b * c.x);
   }
 }
 
@@ -111,8 +173,7 @@ constexpr int kMaxPairBytes = 96 * 1024;   // cosines and sines of a tile
 }  // namespace
 
 int rope_pos_kernels_init() {
-  for (auto k : {rope_pos_tile<true, true>, rope_pos_tile<true, false>, rope_pos_tile<false, true>,
-                 rope_pos_tile<false, false>})
+  for (auto k : {rope_pos_vec<true>, rope_pos_vec<false>, rope_pos_any<true>, rope_pos_any<false>})
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPairBytes) !=
         cudaSuccess) {
       cudaGetLastError();
@@ -121,38 +182,43 @@ int rope_pos_kernels_init() {
   return HEXLIB_B200_OK;
 }
 
-int launch_rope_pos(const RopePosDesc& d, cudaStream_t s) {
+int launch_rope_pos(const RopePosDesc& desc, cudaStream_t s) {
+  RopePosDesc d = desc;
+  if (d.n_axes == 1) d.axis = nullptr;     // every number clamps to 0
   const bool inter = d.layout == HEXLIB_B200_ROPE_INTERLEAVED;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.y) |
                          static_cast<uintptr_t>(2 * d.x_stride) |
                          static_cast<uintptr_t>(2 * d.y_stride) | static_cast<uintptr_t>(2 * d.D);
-  const bool vec = bits % 16 == 0 && d.rot % (inter ? 8 : 16) == 0;
+  const bool vec = bits % 16 == 0 && d.rot % (inter ? 8 : 16) == 0 && d.D <= 4096;
   RopeShape sh;
   sh.pairs = d.rot / 2;
-  sh.rot_items = vec ? sh.pairs / (inter ? 4 : 8) : sh.pairs;
-  sh.items = sh.rot_items + (vec ? (d.D - d.rot) / 8 : d.D - d.rot);
   if ((int64_t)sh.pairs * 8 > kMaxPairBytes) return HEXLIB_B200_ERR_INVAL_PARAMS;
-  // tokens of a CTA: about a cosine for each thread and a few items for each, but no
-  // fewer CTAs than SMs; few tokens split their heads over CTAs instead
+  sh.rot_items = vec ? sh.pairs / (inter ? 4 : 8) : sh.pairs;
+  sh.items = sh.rot_items + (d.x == d.y ? 0 : vec ? (d.D - d.rot) / 8 : d.D - d.rot);
+  // tokens of a CTA: a few cosines and about eight items to a thread, but four CTAs to
+  // an SM where there are tokens for them; few tokens split their heads over CTAs
   const int64_t per_token = (int64_t)d.H * sh.items;
-  int64_t tokens = kThreads / sh.pairs;
-  if (tokens > 4 * kThreads / per_token) tokens = 4 * kThreads / per_token;
-  if (tokens > d.T / 148) tokens = d.T / 148;
+  int64_t tokens = 2 * kThreads / sh.pairs;
+  if (tokens > 8 * kThreads / per_token) tokens = 8 * kThreads / per_token;
+  if (tokens > d.T / (4 * 148)) tokens = d.T / (4 * 148);
   if (tokens < 1) tokens = 1;
   sh.tokens = (int)tokens;
   const int64_t tiles = (d.T + tokens - 1) / tokens;
-  int64_t split = 296 / tiles;
-  if (split > (per_token + kThreads - 1) / kThreads) split = (per_token + kThreads - 1) / kThreads;
+  int64_t split = 296 / tiles, most = (per_token + kThreads - 1) / kThreads;
+  if (split > most) split = most;
+  if (split < (d.H + 1023) / 1024) split = (d.H + 1023) / 1024;   // (items in 32 bits)
   if (split > d.H) split = d.H;
   if (split < 1) split = 1;
   sh.heads = (int)((d.H + split - 1) / split);
   sh.head_split = (d.H + sh.heads - 1) / sh.heads;
   if (tiles * sh.head_split > 0x7fffffff) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  sh.per_item = (uint32_t)(((1ull << 32) + sh.items - 1) / sh.items);
+  sh.per_head = (uint32_t)(((1ull << 32) + sh.heads - 1) / sh.heads);
   const unsigned grid = (unsigned)(tiles * sh.head_split);
   const size_t smem = (size_t)sh.tokens * sh.pairs * sizeof(float2);
   auto go = [&](auto kernel) { kernel<<<grid, kThreads, smem, s>>>(d, sh); };
-  if (vec) inter ? go(rope_pos_tile<true, true>) : go(rope_pos_tile<true, false>);
-  else inter ? go(rope_pos_tile<false, true>) : go(rope_pos_tile<false, false>);
+  if (vec) inter ? go(rope_pos_vec<true>) : go(rope_pos_vec<false>);
+  else inter ? go(rope_pos_any<true>) : go(rope_pos_any<false>);
   if (cudaPeekAtLastError() != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
