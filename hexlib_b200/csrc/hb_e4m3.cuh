@@ -94,6 +94,30 @@ __device__ __forceinline__ uint2 e4m3_encode8(const uint32_t (&w)[4], uint32_t h
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
 
+// The same for a block held by a whole warp, four values to a lane as two words: the
+// lane's four codes, low byte first.
+__device__ __forceinline__ uint32_t e4m3_encode4(uint32_t w0, uint32_t w1, uint32_t& byte) {
+  const uint32_t w[2] = {w0, w1};
+  float f[4], amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+    f[2 * j] = v.x;
+    f[2 * j + 1] = v.y;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (isfinite(f[j])) amax = fmaxf(amax, fabsf(f[j]));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  byte = e4m3_scale_byte(amax);
+  const float inv = e4m3_inverse(byte);
+  uint32_t c = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c |= e4m3_code(f[j], inv) << (8 * j);
+  return c;
+}
+
 // Eight fp16 values from p, as four words of two, in loads of VEC values (VEC = 8 for
 // 16-byte aligned rows down to 1 for any); values from `left` on are zeros. With
 // VEC > 1, `left` is a multiple of VEC.

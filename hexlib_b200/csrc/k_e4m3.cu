@@ -70,19 +70,12 @@ __global__ void __launch_bounds__(kThreads) quantize_weight_e4m3(const __half* _
   __syncthreads();
   for (int c = warp; c < 32 && n0 + c < N; c += kThreads / 32) {
     const int64_t n = n0 + c;
-    float v[4], amax = 0.f;
+    uint32_t w[2], byte;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[j] = __half2float(tile[lane * 4 + j][c]);
-      if (isfinite(v[j])) amax = fmaxf(amax, fabsf(v[j]));
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const uint32_t byte = e4m3_scale_byte(amax);
-    const float inv = e4m3_inverse(byte);
-    uint32_t q = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) q |= e4m3_code(v[j], inv) << (8 * j);
+    for (int j = 0; j < 2; ++j)
+      w[j] = __half_as_ushort(tile[lane * 4 + 2 * j][c]) |
+             ((uint32_t)__half_as_ushort(tile[lane * 4 + 2 * j + 1][c]) << 16);
+    const uint32_t q = e4m3_encode4(w[0], w[1], byte);
     *reinterpret_cast<uint32_t*>(codes + n * (int64_t)blocks * 128 + b * 128 + lane * 4) = q;
     if (lane == 0) scales[e4m3_scale_at(n, b, N)] = (uint8_t)byte;
     if (b == blocks - 1 && lane < padded - blocks)

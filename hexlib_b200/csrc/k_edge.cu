@@ -82,39 +82,85 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <int VEC>
-__device__ __forceinline__ void load8f(float2 (&f)[4], const float* p, int left) {
-  if constexpr (VEC == 8) {
-    const float4 a = left > 0 ? __ldg(reinterpret_cast<const float4*>(p)) : make_float4(0, 0, 0, 0);
-    const float4 b = left > 0 ? __ldg(reinterpret_cast<const float4*>(p) + 1) : make_float4(0, 0, 0, 0);
-    f[0] = make_float2(a.x, a.y);
-    f[1] = make_float2(a.z, a.w);
-    f[2] = make_float2(b.x, b.y);
-    f[3] = make_float2(b.z, b.w);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      f[q] = make_float2(2 * q < left ? __ldg(p + 2 * q) : 0.f,
-                         2 * q + 1 < left ? __ldg(p + 2 * q + 1) : 0.f);
+// The columns of a thread. With rows of whole 16-byte vectors (WIDE), vector j of thread
+// g is columns (j G + g) 8 to + 7, so 16 threads hold a block of 128. Otherwise a WARP
+// holds a block, element i of a lane 32 (i % 4) further, so that scalar accesses of a
+// warp are consecutive (1001 rows of 1203: 15 us with the first order and scalar
+// accesses, 6.4 with this one).
+template <int G, bool WIDE>
+struct Columns {
+  int base;                                          // of element 0 of vector 0
+  __device__ Columns() {
+    const int g = G == 32 ? (threadIdx.x & 31) : threadIdx.x;
+    base = WIDE ? g * 8 : (G == 32 ? 0 : (g >> 5) * 128) + (g & 31);
   }
-}
-// A pair with zeros from `left` on. With VEC 8 a vector is in the row or not, which the
-// callers know.
-template <int VEC>
-__device__ __forceinline__ uint32_t pack_in(float2 f, int q, int left) {
-  if constexpr (VEC == 8) return pack(f.x, f.y);
-  return pack(2 * q < left ? f.x : 0.f, 2 * q + 1 < left ? f.y : 0.f);
-}
+  // from its first column, a constant once the loops are unrolled; rows below start there
+  static __device__ __forceinline__ int off(int j, int i) {
+    return WIDE ? j * G * 8 + i : (2 * j + (i >> 2)) * (G / 32) * 128 + (i & 3) * 32;
+  }
+  __device__ __forceinline__ int at(int j, int i) const { return base + off(j, i); }
+
+  __device__ __forceinline__ void load(uint32_t (&w)[4], const __half* row, int j, int C) const {
+    if constexpr (WIDE) {
+      load8<8>(w, row + off(j, 0), C - at(j, 0));
+    } else {
+      const unsigned short* p = reinterpret_cast<const unsigned short*>(row);
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        w[q] = (at(j, 2 * q) < C ? (uint32_t)p[off(j, 2 * q)] : 0u) |
+               (at(j, 2 * q + 1) < C ? (uint32_t)p[off(j, 2 * q + 1)] << 16 : 0u);
+    }
+  }
+  __device__ __forceinline__ void store(__half* row, const uint32_t (&w)[4], int j, int C) const {
+    if constexpr (WIDE) {
+      store8<8>(row + off(j, 0), w, C - at(j, 0));
+    } else {
+      unsigned short* p = reinterpret_cast<unsigned short*>(row);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (at(j, 2 * q) < C) p[off(j, 2 * q)] = (unsigned short)w[q];
+        if (at(j, 2 * q + 1) < C) p[off(j, 2 * q + 1)] = (unsigned short)(w[q] >> 16);
+      }
+    }
+  }
+  __device__ __forceinline__ void load(float2 (&f)[4], const float* row, int j, int C) const {
+    if constexpr (WIDE) {
+      const float4* p = reinterpret_cast<const float4*>(row + off(j, 0));
+      const bool in = at(j, 0) < C;
+      const float4 a = in ? __ldg(p) : make_float4(0, 0, 0, 0);
+      const float4 b = in ? __ldg(p + 1) : make_float4(0, 0, 0, 0);
+      f[0] = make_float2(a.x, a.y);
+      f[1] = make_float2(a.z, a.w);
+      f[2] = make_float2(b.x, b.y);
+      f[3] = make_float2(b.z, b.w);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        f[q] = make_float2(at(j, 2 * q) < C ? __ldg(row + off(j, 2 * q)) : 0.f,
+                           at(j, 2 * q + 1) < C ? __ldg(row + off(j, 2 * q + 1)) : 0.f);
+    }
+  }
+  // a vector past C, as zeros
+  __device__ __forceinline__ void zero_out(uint32_t (&w)[4], int j, int C) const {
+    if (WIDE && at(j, 0) >= C) w[0] = w[1] = w[2] = w[3] = 0;
+  }
+  // a pair with zeros past C, where a vector may end within the row
+  __device__ __forceinline__ uint32_t pack_in(float2 f, int j, int q, int C) const {
+    const uint32_t w = pack(f.x, f.y);
+    if constexpr (WIDE) return w;                    // the vector is in or not: see zero_out
+    return (at(j, 2 * q) < C ? w & 0xffffu : 0u) | (at(j, 2 * q + 1) < C ? w & 0xffff0000u : 0u);
+  }
+};
 
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// A row in the registers of the G threads that share it, as floats: vector j of thread
-// g is columns (j G + g) 8 and on, zeros past C. Each step runs over all V vectors
+// A row in the registers of the G threads that share it, as floats, zeros past C. Each step runs over all V vectors
 // between two branches, so that their chains overlap, in two-wide instructions with
 // every rounding written out: the fp16 and the 8-bit form give the same bits.
-template <int G, int V, int VEC>
+template <int G, int V, bool WIDE>
 struct Row {
   float2 v[V][4];
+  Columns<G, WIDE> col;
 
   __device__ __forceinline__ void unpack(const uint32_t (&w)[V][4]) {
 #pragma unroll
@@ -125,7 +171,7 @@ struct Row {
 
   // norm(v) w + b, the moments taken over the whole row (the squared deviations of a
   // layer norm after its mean). v inv - mean inv is one fused step a pair.
-  __device__ __forceinline__ void norm(const float* w, const float* b, int g, int C, float per_c,
+  __device__ __forceinline__ void norm(const float* w, const float* b, int C, float per_c,
                                        bool layer, float eps, RowSum<G>& sum) {
     float2 ss = both(0.f);
     float mean = 0.f;
@@ -137,16 +183,14 @@ struct Row {
         for (int q = 0; q < 4; ++q) s = __fadd2_rn(s, v[j][q]);
       mean = sum(s.x + s.y) * per_c;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int left = C - (j * G + g) * 8;
+      for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           float2 d = __fadd2_rn(v[j][q], both(-mean));
-          if ((VEC == 8 ? 0 : 2 * q) >= left) d.x = 0.f;
-          if ((VEC == 8 ? 0 : 2 * q + 1) >= left) d.y = 0.f;
+          if (col.at(j, WIDE ? 0 : 2 * q) >= C) d.x = 0.f;
+          if (col.at(j, WIDE ? 0 : 2 * q + 1) >= C) d.y = 0.f;
           ss = __ffma2_rn(d, d, ss);
         }
-      }
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j)
@@ -158,10 +202,9 @@ struct Row {
     if (b) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int c = (j * G + g) * 8;
         float2 wv[4], bv[4];
-        load8f<VEC>(wv, w + c, C - c);
-        load8f<VEC>(bv, b + c, C - c);
+        col.load(wv, w + col.base, j, C);
+        col.load(bv, b + col.base, j, C);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           v[j][q] = __ffma2_rn(__ffma2_rn(v[j][q], both(inv), shift), wv[q], bv[q]);
@@ -169,9 +212,8 @@ struct Row {
     } else {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int c = (j * G + g) * 8;
         float2 wv[4];
-        load8f<VEC>(wv, w + c, C - c);
+        col.load(wv, w + col.base, j, C);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           v[j][q] = __fmul2_rn(__ffma2_rn(v[j][q], both(inv), shift), wv[q]);
@@ -200,75 +242,87 @@ constexpr int held_threads(int G) { return G == 32 ? 128 : G; }
 constexpr int held_ctas(int G, int V) {       // of an SM: registers for V vectors of x, y, gate
   return (V == 1 ? 1024 : V == 2 ? 768 : V == 3 ? 640 : V == 4 ? 512 : 256) / held_threads(G);
 }
-template <int G, int V, int VEC, bool E4M3>
+template <int G, int V, bool WIDE, bool E4M3>
 __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(const EdgeDesc d) {
   __shared__ __align__(16) float red[4][8];
   RowSum<G> sum{red};
   constexpr int ROWS = G == 32 ? held_threads(G) / 32 : 1;
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
-  const int g = G == 32 ? (threadIdx.x & 31) : threadIdx.x;
   const int per_gate = d.gate ? d.R / d.gate_rows : 1;
   const int C = d.C, blocks = (C + 127) / 128, padded = (blocks + 3) / 4 * 4;
   const float per_c = 1.f / C;
   const int64_t step = (int64_t)gridDim.x * ROWS;
+  const Columns<G, WIDE> col;
   for (int64_t r = blockIdx.x * (int64_t)ROWS + (G == 32 ? threadIdx.x >> 5 : 0); r < d.R;
        r += step) {
-    const int64_t at = r * C + g * 8;             // of vector 0; vector j is G * 8 further
+    Row<G, V, WIDE> v;
+    const int64_t at = r * C + col.base;
     uint32_t x[V][4];
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      load8<VEC>(x[j], (const __half*)d.x + at + j * G * 8, C - (j * G + g) * 8);
-    Row<G, V, VEC> v;
+    for (int j = 0; j < V; ++j) col.load(x[j], (const __half*)d.x + at, j, C);
     if (d.y) {
       uint32_t y[V][4], gate[V][4];
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        load8<VEC>(y[j], (const __half*)d.y + at + j * G * 8, C - (j * G + g) * 8);
+      for (int j = 0; j < V; ++j) col.load(y[j], (const __half*)d.y + at, j, C);
       if (d.gate) {
-        const __half* gp = (const __half*)d.gate + (int64_t)((int)r / per_gate) * C + g * 8;
+        const __half* gp =
+            (const __half*)d.gate + (int64_t)((int)r / per_gate) * C + col.base;
 #pragma unroll
-        for (int j = 0; j < V; ++j) load8<VEC>(gate[j], gp + j * G * 8, C - (j * G + g) * 8);
+        for (int j = 0; j < V; ++j) col.load(gate[j], gp, j, C);
       }
       v.unpack(y);
-      if (d.post_w) v.norm(d.post_w, d.post_b, g, C, per_c, layer, d.eps, sum);
+      if (d.post_w) v.norm(d.post_w, d.post_b, C, per_c, layer, d.eps, sum);
       if (d.gate) v.gated(gate, d.gate_act);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int left = C - (j * G + g) * 8;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          x[j][q] = pack_in<VEC>(__ffma2_rn(both(d.x_scale), halves(x[j][q]),
-                                            __fmul2_rn(both(d.y_scale), v.v[j][q])), q, left);
-        store8<VEC>((__half*)d.x_out + at + j * G * 8, x[j], left);
-        if (VEC == 8 && left <= 0) x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0;
+          x[j][q] = col.pack_in(__ffma2_rn(both(d.x_scale), halves(x[j][q]),
+                                           __fmul2_rn(both(d.y_scale), v.v[j][q])), j, q, C);
+        col.store((__half*)d.x_out + at, x[j], j, C);
+        col.zero_out(x[j], j, C);
       }
     }
     if (!d.pre_w) continue;
     v.unpack(x);
-    v.norm(d.pre_w, d.pre_b, g, C, per_c, layer, d.eps, sum);
+    v.norm(d.pre_w, d.pre_b, C, per_c, layer, d.eps, sum);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (j * G + g) * 8;
       uint32_t h[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) h[q] = pack_in<VEC>(v.v[j][q], q, C - c);
+      for (int q = 0; q < 4; ++q) h[q] = col.pack_in(v.v[j][q], j, q, C);
       if constexpr (!E4M3) {
-        store8<VEC>((__half*)d.h + at + j * G * 8, h, C - c);
-      } else {
+        col.store((__half*)d.h + at, h, j, C);
+      } else if constexpr (WIDE) {
         // 16 consecutive threads hold a block; blocks past the last are zeros
-        const int b128 = c >> 7;
-        if (VEC == 8 && c >= C) h[0] = h[1] = h[2] = h[3] = 0;
+        const int c = col.at(j, 0), b128 = c >> 7;
+        col.zero_out(h, j, C);
         uint32_t byte;
         const uint2 codes = e4m3_encode8(h, 0xffffu << (threadIdx.x & 16), byte);
         if (b128 < blocks)
           *reinterpret_cast<uint2*>((uint8_t*)d.h_codes + r * (int64_t)blocks * 128 + c) = codes;
         if ((threadIdx.x & 15) == 0 && b128 < padded)
           ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b128, d.R)] = (uint8_t)byte;
+      } else {
+        // the warp holds two blocks, four values of each to a lane
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int c = col.at(j, 4 * k), b128 = c >> 7;
+          uint32_t byte;
+          const uint32_t codes = e4m3_encode4(h[2 * k], h[2 * k + 1], byte);
+          if (b128 < blocks) {
+            uint8_t* to = (uint8_t*)d.h_codes + r * (int64_t)blocks * 128 + c;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i * 32] = (uint8_t)(codes >> (8 * i));
+          }
+          if ((threadIdx.x & 31) == 0 && b128 < padded)
+            ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b128, d.R)] = (uint8_t)byte;
+        }
       }
     }
     if constexpr (E4M3) {
       // scale bytes of the last word that no thread's columns reach
-      for (int b = G * V / 16 + g; b < padded; b += G)
+      for (int b = G * V / 16 + (G == 32 ? threadIdx.x & 31 : threadIdx.x); b < padded; b += G)
         ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b, d.R)] = (uint8_t)kE4m3One;
     }
   }
@@ -367,10 +421,10 @@ int with_layout(int C, F&& f) {
 
 // CTAs of a form that are resident on the device at once, found when it is loaded (a
 // grid of more would leave a partial last wave: 1184 CTAs on 444 measured 11 % slower).
-template <int G, int V, int VEC, bool E4M3>
+template <int G, int V, bool WIDE, bool E4M3>
 std::atomic<int> g_resident{0};
 
-template <int VEC, bool E4M3>
+template <bool WIDE, bool E4M3>
 int launch_form(const EdgeDesc& d, cudaStream_t s) {
   return with_layout(d.C, [&](auto G, auto V) {
     if constexpr (G.value == 0) {
@@ -378,8 +432,8 @@ int launch_form(const EdgeDesc& d, cudaStream_t s) {
     } else {
       const int64_t rows = G.value == 32 ? held_threads(32) / 32 : 1;
       const int64_t ctas = (d.R + rows - 1) / rows;
-      const int64_t most = g_resident<G.value, V.value, VEC, E4M3>.load(std::memory_order_relaxed);
-      edge_held<G.value, V.value, VEC, E4M3>
+      const int64_t most = g_resident<G.value, V.value, WIDE, E4M3>.load(std::memory_order_relaxed);
+      edge_held<G.value, V.value, WIDE, E4M3>
           <<<(unsigned)(ctas < most ? ctas : most), held_threads(G.value), 0, s>>>(d);
     }
     if (cudaPeekAtLastError() != cudaSuccess) {
@@ -390,7 +444,7 @@ int launch_form(const EdgeDesc& d, cudaStream_t s) {
   });
 }
 
-template <int VEC, bool E4M3>
+template <bool WIDE, bool E4M3>
 bool load_form(int sms) {
   cudaFuncAttributes a;
   bool ok = cudaFuncGetAttributes(&a, (const void*)edge_wide<E4M3>) == cudaSuccess;
@@ -399,9 +453,9 @@ bool load_form(int sms) {
       if constexpr (G.value != 0) {
         int n = 0;
         ok = ok && cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-                       &n, (const void*)edge_held<G.value, V.value, VEC, E4M3>,
+                       &n, (const void*)edge_held<G.value, V.value, WIDE, E4M3>,
                        held_threads(G.value), 0) == cudaSuccess && n > 0;
-        g_resident<G.value, V.value, VEC, E4M3>.store(n * sms, std::memory_order_relaxed);
+        g_resident<G.value, V.value, WIDE, E4M3>.store(n * sms, std::memory_order_relaxed);
       }
       return 0;
     });
@@ -415,8 +469,8 @@ int edge_kernels_init() {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-      !load_form<8, false>(sms) || !load_form<8, true>(sms) || !load_form<1, false>(sms) ||
-      !load_form<1, true>(sms)) {
+      !load_form<true, false>(sms) || !load_form<true, true>(sms) || !load_form<false, false>(sms) ||
+      !load_form<false, true>(sms)) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
@@ -430,8 +484,8 @@ int launch_edge(const EdgeDesc& d, cudaStream_t s) {
                         (const void*)d.post_b})
     bits |= reinterpret_cast<uintptr_t>(p);
   const bool wide = bits % 16 == 0;
-  if (d.h_codes) return wide ? launch_form<8, true>(d, s) : launch_form<1, true>(d, s);
-  return wide ? launch_form<8, false>(d, s) : launch_form<1, false>(d, s);
+  if (d.h_codes) return wide ? launch_form<true, true>(d, s) : launch_form<false, true>(d, s);
+  return wide ? launch_form<true, false>(d, s) : launch_form<false, false>(d, s);
 }
 
 }  // namespace hb
