@@ -497,7 +497,7 @@ int hexlib_b200_matmul_epilogue_residual_e4m3(const void* a_codes, const void* a
   return matmul_e4m3(a_codes, a_scales, w_codes, w_scales, bias, r, out, M, K, N, act, stream);
 }
 
-static int edge(const hb::EdgeDesc& d, bool e4m3, void* stream) {
+static int edge(hb::EdgeDesc& d, bool e4m3, void* stream) {
   if (d.R < 0 || d.C <= 0 || (d.norm != HEXLIB_B200_NORM_RMS && d.norm != HEXLIB_B200_NORM_LAYER) ||
       !(d.eps >= 0.f) || d.gate_act < HEXLIB_B200_GATE_NONE || d.gate_act > HEXLIB_B200_GATE_TANH)
     return HEXLIB_B200_ERR_INVAL_PARAMS;
@@ -523,6 +523,7 @@ static int edge(const hb::EdgeDesc& d, bool e4m3, void* stream) {
   for (const void* p : {d.x, d.y, d.gate, static_cast<const void*>(d.x_out)})
     if (shares(p, d.h_codes) || shares(p, d.h_scales)) return HEXLIB_B200_ERR_INVAL_PARAMS;
   HB_ENTRY_INIT();
+  d.err = hb::default_error_word();
   return hb::launch_edge(d, as_stream(stream));
 }
 

@@ -321,6 +321,16 @@ __device__ __forceinline__ void tma_load_2d(const CUtensorMap* map, uint64_t* ba
       : "memory");
 }
 
+// Untiled bulk load: both addresses 16-byte aligned, the size a multiple of 16.
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(smem_dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // Bulk tensor store shared::cta -> global, tracked by bulk async-groups.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map,
                                              const void* smem_src, int c0,

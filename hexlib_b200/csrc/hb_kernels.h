@@ -181,6 +181,7 @@ struct EdgeDesc {
   void* h_scales;
   int R, C, norm;
   float eps;
+  int* err;                 // error word of bounded waits
 };
 int edge_kernels_init();
 int launch_edge(const EdgeDesc& d, cudaStream_t s);

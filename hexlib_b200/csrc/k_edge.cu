@@ -9,6 +9,7 @@
 #include <atomic>
 #include <type_traits>
 
+#include "hb_device.cuh"
 #include "hb_e4m3.cuh"
 #include "hb_kernels.h"
 
@@ -48,6 +49,15 @@ __device__ __forceinline__ float normed(float v, float2 ms, float w, float b) {
 }
 __device__ __forceinline__ float blended(float x_scale, float x, float y_scale, float u) {
   return fmaf(x_scale, x, __fmul_rn(y_scale, u));
+}
+
+// 1 / sqrt(a): rsqrtf (2 ulp) and one Newton step, which leaves its own rounding. Every
+// value of the row carries this error, and with it one in 2^18 codes of the 8-bit form
+// fell on the other side of a tie.
+__device__ __forceinline__ float inverse_root(float a) {
+  const float y = rsqrtf(a);
+  const float e = fmaf(-__fmul_rn(a, y), y, 1.f);
+  return a < INFINITY ? fmaf(0.5f * y, e, y) : y;
 }
 
 // Sum over the G threads of a row: a warp, or the CTA of G threads through shared
@@ -197,13 +207,29 @@ struct Row {
 #pragma unroll
         for (int q = 0; q < 4; ++q) ss = __ffma2_rn(v[j][q], v[j][q], ss);
     }
-    const float inv = rsqrtf(fmaf(sum(ss.x + ss.y), per_c, eps));
+    // the weights of a row by a CTA are read ahead of the sum's barrier (a warp's own row
+    // has none, and registers to lose)
+    constexpr bool AHEAD = G > 32;
+    float2 ahead[AHEAD ? V : 1][4];
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) col.load(ahead[j], w + col.base, j, C);
+    }
+    auto weights = [&](int j, float2 (&wv)[4]) {
+      if constexpr (AHEAD) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) wv[q] = ahead[j][q];
+      } else {
+        col.load(wv, w + col.base, j, C);
+      }
+    };
+    const float inv = inverse_root(fmaf(sum(ss.x + ss.y), per_c, eps));
     const float2 shift = both(-__fmul_rn(mean, inv));
     if (b) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float2 wv[4], bv[4];
-        col.load(wv, w + col.base, j, C);
+        weights(j, wv);
         col.load(bv, b + col.base, j, C);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -213,7 +239,7 @@ struct Row {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float2 wv[4];
-        col.load(wv, w + col.base, j, C);
+        weights(j, wv);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           v[j][q] = __fmul2_rn(__ffma2_rn(v[j][q], both(inv), shift), wv[q]);
@@ -221,13 +247,17 @@ struct Row {
     }
   }
 
-  // v *= f(gate)
-  __device__ __forceinline__ void gated(const uint32_t (&gate)[V][4], int act) {
+  // v *= f(gate), vector j of the gate being gate(j, w)
+  template <class Gate>
+  __device__ __forceinline__ void gated(Gate gate, int act) {
     auto times = [&](auto f) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
+      for (int j = 0; j < V; ++j) {
+        uint32_t w[4];
+        gate(j, w);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[j][q] = __fmul2_rn(v[j][q], f(halves(gate[j][q])));
+        for (int q = 0; q < 4; ++q) v[j][q] = __fmul2_rn(v[j][q], f(halves(w[q])));
+      }
     };
     if (act == HEXLIB_B200_GATE_NONE) times([](float2 x) { return x; });
     else if (act == HEXLIB_B200_GATE_SIGMOID) times([](float2 x) { return sigmoid2(x); });
@@ -235,6 +265,53 @@ struct Row {
     else times([](float2 x) { return make_float2(tanhf(x.x), tanhf(x.y)); });
   }
 };
+
+// h of row r from the normed row v, in fp16 or in its e4m3 form.
+template <int G, int V, bool WIDE, bool E4M3>
+__device__ __forceinline__ void write_h(const EdgeDesc& d, const Row<G, V, WIDE>& v, int64_t r) {
+  const Columns<G, WIDE>& col = v.col;
+  const int C = d.C, blocks = (C + 127) / 128, padded = (blocks + 3) / 4 * 4;
+  const int64_t at = r * C + col.base;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    uint32_t h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) h[q] = col.pack_in(v.v[j][q], j, q, C);
+    if constexpr (!E4M3) {
+      col.store((__half*)d.h + at, h, j, C);
+    } else if constexpr (WIDE) {
+      // 16 consecutive threads hold a block; blocks past the last are zeros
+      const int c = col.at(j, 0), b128 = c >> 7;
+      col.zero_out(h, j, C);
+      uint32_t byte;
+      const uint2 codes = e4m3_encode8(h, 0xffffu << (threadIdx.x & 16), byte);
+      if (b128 < blocks)
+        *reinterpret_cast<uint2*>((uint8_t*)d.h_codes + r * (int64_t)blocks * 128 + c) = codes;
+      if ((threadIdx.x & 15) == 0 && b128 < padded)
+        ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b128, d.R)] = (uint8_t)byte;
+    } else {
+      // the warp holds two blocks, four values of each to a lane
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int c = col.at(j, 4 * k), b128 = c >> 7;
+        uint32_t byte;
+        const uint32_t codes = e4m3_encode4(h[2 * k], h[2 * k + 1], byte);
+        if (b128 < blocks) {
+          uint8_t* to = (uint8_t*)d.h_codes + r * (int64_t)blocks * 128 + c;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) to[i * 32] = (uint8_t)(codes >> (8 * i));
+        }
+        if ((threadIdx.x & 31) == 0 && b128 < padded)
+          ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b128, d.R)] = (uint8_t)byte;
+      }
+    }
+  }
+  if constexpr (E4M3) {
+    // scale bytes of the last word that no thread's columns reach
+    for (int b = G * V / 16 + (G == 32 ? threadIdx.x & 31 : threadIdx.x); b < padded; b += G)
+      ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b, d.R)] = (uint8_t)kE4m3One;
+  }
+}
 
 // A row of up to G * V * 8 values in the registers of G threads (a warp, or the CTA),
 // read once and written once; its gate is read with it, ahead of the sums.
@@ -249,7 +326,7 @@ __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(co
   constexpr int ROWS = G == 32 ? held_threads(G) / 32 : 1;
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
   const int per_gate = d.gate ? d.R / d.gate_rows : 1;
-  const int C = d.C, blocks = (C + 127) / 128, padded = (blocks + 3) / 4 * 4;
+  const int C = d.C;
   const float per_c = 1.f / C;
   const int64_t step = (int64_t)gridDim.x * ROWS;
   const Columns<G, WIDE> col;
@@ -272,7 +349,11 @@ __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(co
       }
       v.unpack(y);
       if (d.post_w) v.norm(d.post_w, d.post_b, C, per_c, layer, d.eps, sum);
-      if (d.gate) v.gated(gate, d.gate_act);
+      if (d.gate)
+        v.gated([&](int j, uint32_t (&w)[4]) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) w[q] = gate[j][q];
+        }, d.gate_act);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
 #pragma unroll
@@ -286,45 +367,80 @@ __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(co
     if (!d.pre_w) continue;
     v.unpack(x);
     v.norm(d.pre_w, d.pre_b, C, per_c, layer, d.eps, sum);
+    write_h<G, V, WIDE, E4M3>(d, v, r);
+  }
+}
+
+// Wide rows of whole vectors, one CTA of G threads to a row: the bulk copy engine brings
+// x, y and the gate of the next row to shared memory while the norm before the next
+// block and the codes of this one are computed, so no warp waits for memory with its
+// registers full, and more of them fit (16384 x 4096 with a sigmoid gate for each element
+// and 8-bit h: 121 us, 5.0 TB/s; 140 with the rows loaded to registers, 134 with 128
+// threads of four vectors to a row).
+constexpr int row_ctas(int G, int V) {
+  return G == 128 ? (V == 2 ? 8 : 6) : V == 2 ? 4 : V <= 4 ? 3 : 1;
+}
+template <int G, int V, bool E4M3>
+__global__ void __launch_bounds__(G, row_ctas(G, V)) edge_row(const EdgeDesc d) {
+  extern __shared__ __align__(16) __half rows[];     // x, y, gate of a row
+  __shared__ __align__(16) float red[4][8];
+  __shared__ uint64_t full;
+  __shared__ int abort_flag;
+  RowSum<G> sum{red};
+  const Columns<G, true> col;
+  const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
+  const int per_gate = d.gate ? d.R / d.gate_rows : 1;
+  const int C = d.C;
+  const float per_c = 1.f / C;
+  const uint32_t bytes = C * 2;
+  auto bring = [&](int r) {                          // by thread 0
+    mbar_arrive_expect_tx(&full, bytes * (1 + (d.y != nullptr) + (d.gate != nullptr)));
+    bulk_load(rows, (const __half*)d.x + (int64_t)r * C, bytes, &full);
+    if (d.y) bulk_load(rows + C, (const __half*)d.y + (int64_t)r * C, bytes, &full);
+    if (d.gate)
+      bulk_load(rows + 2 * C, (const __half*)d.gate + (int64_t)(r / per_gate) * C, bytes, &full);
+  };
+  if (threadIdx.x == 0) {
+    mbar_init(&full, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+    bring(blockIdx.x);
+  }
+  __syncthreads();
+  uint32_t phase = 0;
+  for (int r = blockIdx.x; r < d.R; r += gridDim.x, phase ^= 1u) {
+    if (!__syncthreads_and(mbar_wait(&full, phase, &abort_flag, d.err))) return;
+    const int64_t at = (int64_t)r * C + col.base;
+    Row<G, V, true> v;
+    uint32_t x[V][4];
+    if (d.y) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      uint32_t h[4];
+      for (int j = 0; j < V; ++j) col.load(x[j], rows + C + col.base, j, C);
+      v.unpack(x);
+      if (d.post_w) v.norm(d.post_w, d.post_b, C, per_c, layer, d.eps, sum);
+      if (d.gate)
+        v.gated([&](int j, uint32_t (&w)[4]) { col.load(w, rows + 2 * C + col.base, j, C); },
+                d.gate_act);
+    }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) h[q] = col.pack_in(v.v[j][q], j, q, C);
-      if constexpr (!E4M3) {
-        col.store((__half*)d.h + at, h, j, C);
-      } else if constexpr (WIDE) {
-        // 16 consecutive threads hold a block; blocks past the last are zeros
-        const int c = col.at(j, 0), b128 = c >> 7;
-        col.zero_out(h, j, C);
-        uint32_t byte;
-        const uint2 codes = e4m3_encode8(h, 0xffffu << (threadIdx.x & 16), byte);
-        if (b128 < blocks)
-          *reinterpret_cast<uint2*>((uint8_t*)d.h_codes + r * (int64_t)blocks * 128 + c) = codes;
-        if ((threadIdx.x & 15) == 0 && b128 < padded)
-          ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b128, d.R)] = (uint8_t)byte;
-      } else {
-        // the warp holds two blocks, four values of each to a lane
+    for (int j = 0; j < V; ++j) col.load(x[j], rows + col.base, j, C);
+    __syncthreads();                                 // the row has been read
+    if (threadIdx.x == 0 && r + (int)gridDim.x < d.R) bring(r + gridDim.x);
+    if (d.y) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int c = col.at(j, 4 * k), b128 = c >> 7;
-          uint32_t byte;
-          const uint32_t codes = e4m3_encode4(h[2 * k], h[2 * k + 1], byte);
-          if (b128 < blocks) {
-            uint8_t* to = (uint8_t*)d.h_codes + r * (int64_t)blocks * 128 + c;
+      for (int j = 0; j < V; ++j) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[i * 32] = (uint8_t)(codes >> (8 * i));
-          }
-          if ((threadIdx.x & 31) == 0 && b128 < padded)
-            ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b128, d.R)] = (uint8_t)byte;
-        }
+        for (int q = 0; q < 4; ++q)
+          x[j][q] = col.pack_in(__ffma2_rn(both(d.x_scale), halves(x[j][q]),
+                                           __fmul2_rn(both(d.y_scale), v.v[j][q])), j, q, C);
+        col.store((__half*)d.x_out + at, x[j], j, C);
+        col.zero_out(x[j], j, C);
       }
     }
-    if constexpr (E4M3) {
-      // scale bytes of the last word that no thread's columns reach
-      for (int b = G * V / 16 + (G == 32 ? threadIdx.x & 31 : threadIdx.x); b < padded; b += G)
-        ((uint8_t*)d.h_scales)[e4m3_scale_at(r, b, d.R)] = (uint8_t)kE4m3One;
-    }
+    if (!d.pre_w) continue;
+    v.unpack(x);
+    v.norm(d.pre_w, d.pre_b, C, per_c, layer, d.eps, sum);
+    write_h<G, V, true, E4M3>(d, v, r);
   }
 }
 
@@ -343,7 +459,7 @@ __device__ __forceinline__ float2 moments_wide(const __half* v, int C, float per
     const float d = __half2float(v[c]) - mean;
     ss = fmaf(d, d, ss);
   }
-  return make_float2(mean, rsqrtf(fmaf(sum(ss), per_c, eps)));
+  return make_float2(mean, inverse_root(fmaf(sum(ss), per_c, eps)));
 }
 
 template <bool E4M3>
@@ -411,7 +527,7 @@ int with_layout(int C, F&& f) {
   HB_EDGE_LAYOUT(32, 4)
   HB_EDGE_LAYOUT(128, 2)
   HB_EDGE_LAYOUT(128, 3)
-  HB_EDGE_LAYOUT(128, 4)
+  HB_EDGE_LAYOUT(256, 2)
   HB_EDGE_LAYOUT(256, 3)
   HB_EDGE_LAYOUT(256, 4)
   HB_EDGE_LAYOUT(256, 8)
@@ -424,6 +540,9 @@ int with_layout(int C, F&& f) {
 template <int G, int V, bool WIDE, bool E4M3>
 std::atomic<int> g_resident{0};
 
+constexpr bool by_row(int G, bool wide) { return wide && G > 32; }
+constexpr int row_bytes(int C) { return 3 * 2 * C; }
+
 template <bool WIDE, bool E4M3>
 int launch_form(const EdgeDesc& d, cudaStream_t s) {
   return with_layout(d.C, [&](auto G, auto V) {
@@ -433,8 +552,11 @@ int launch_form(const EdgeDesc& d, cudaStream_t s) {
       const int64_t rows = G.value == 32 ? held_threads(32) / 32 : 1;
       const int64_t ctas = (d.R + rows - 1) / rows;
       const int64_t most = g_resident<G.value, V.value, WIDE, E4M3>.load(std::memory_order_relaxed);
-      edge_held<G.value, V.value, WIDE, E4M3>
-          <<<(unsigned)(ctas < most ? ctas : most), held_threads(G.value), 0, s>>>(d);
+      const unsigned grid = (unsigned)(ctas < most ? ctas : most);
+      if constexpr (by_row(G.value, WIDE))
+        edge_row<G.value, V.value, E4M3><<<grid, G.value, row_bytes(d.C), s>>>(d);
+      else
+        edge_held<G.value, V.value, WIDE, E4M3><<<grid, held_threads(G.value), 0, s>>>(d);
     }
     if (cudaPeekAtLastError() != cudaSuccess) {
       cudaGetLastError();
@@ -452,9 +574,19 @@ bool load_form(int sms) {
     with_layout(C, [&](auto G, auto V) {
       if constexpr (G.value != 0) {
         int n = 0;
-        ok = ok && cudaOccupancyMaxActiveBlocksPerMultiprocessor(
-                       &n, (const void*)edge_held<G.value, V.value, WIDE, E4M3>,
-                       held_threads(G.value), 0) == cudaSuccess && n > 0;
+        if constexpr (by_row(G.value, WIDE)) {
+          // for the layout's widest row: narrower ones leave no more than a CTA's room unused
+          const int most = row_bytes(G.value * V.value * 8);
+          auto* k = edge_row<G.value, V.value, E4M3>;
+          ok = ok && cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most) ==
+                         cudaSuccess &&
+               cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k, G.value, most) == cudaSuccess;
+        } else {
+          ok = ok && cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+                         &n, (const void*)edge_held<G.value, V.value, WIDE, E4M3>,
+                         held_threads(G.value), 0) == cudaSuccess;
+        }
+        ok = ok && n > 0;
         g_resident<G.value, V.value, WIDE, E4M3>.store(n * sms, std::memory_order_relaxed);
       }
       return 0;
