@@ -2,8 +2,8 @@
 //
 // cuTensorMapEncodeTiled is a driver-API function; it is fetched once through
 // cudaGetDriverEntryPoint so the library links only against the runtime.
-// Every map here is 3-D fp16 (x innermost, then y, then a batch z) with the
-// 128-byte swizzle, and the host checks the encoder's own preconditions
+// The maps are 3-D fp16 (x innermost, then y, then a batch z) or 2-D bytes, with
+// the 128-byte swizzle, and the host checks the encoder's own preconditions
 // (16-byte-aligned base, strides multiple of 16 bytes) before calling it, so a
 // shape TMA cannot describe is refused on the host and never reaches a kernel.
 #pragma once
