@@ -370,7 +370,7 @@ int launch_tile(const GemmE4m3Desc& g, int split_log2, int* err, cudaStream_t s)
 // Epilogue: 8 warps, each 32 rows by 128 columns, 32 columns at a time: from tensor
 // memory through registers and a 2 KiB box in shared memory to rows of 64 bytes, stored
 // by the LSU at any alignment.
-constexpr int kPairThreads = 352;   // loads, MMAs, scales, 8 epilogue warps
+constexpr int kPairThreads = 384;   // loads, MMAs, 2 warps of scales, 8 of epilogue
 
 struct PairCfg {
   static constexpr int BN = 256;
@@ -616,46 +616,49 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
       }
     }
-  } else if (warp == 2) {
-    // scale words of 512 of K: row lane + 32 j of the tile to word j of row `lane`
-    const uint32_t sf_full_lead = cluster_addr(sf_full, 0);
+  } else if (warp <= 3) {
+    // Scale words of 512 of K: row lane + 32 j of the tile to word j of row `lane`. A word
+    // takes its loads, the fence and the arrival one after the other, longer than its
+    // MMAs at two words a tile; so two warps take turns, each with a buffer of its own.
+    const uint32_t b = warp - 2, sf_full_lead = cluster_addr(sf_full + b, 0);
     const int groups = (p.num_kb + 3) >> 2;
-    uint32_t u = 0;
+    uint32_t ph = 1, mine = b;                       // words until this warp's next
     for (; t.left; t.next()) {
-      const int m0 = t.m * 256 + rank * 128, n0 = t.n * BN;
-      for (int g = 0; g < groups; ++g, ++u) {
+      const int m0 = t.m * 256 + rank * 128 + lane, n0 = t.n * BN + lane;
+      for (int g = 0; g < groups; ++g) {
+        if (mine-- != 0) continue;
+        mine = 1;
         uint32_t a[4], w[8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int m = m0 + lane + 32 * j;
-          a[j] = m < p.M ? __ldg(p.a_scales + (int64_t)g * p.M + m) : 0x7f7f7f7fu;
-        }
+        for (int j = 0; j < 4; ++j)
+          a[j] = m0 + 32 * j < p.M ? __ldg(p.a_scales + (int64_t)g * p.M + m0 + 32 * j)
+                                   : 0x7f7f7f7fu;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int n = n0 + lane + 32 * j;
-          w[j] = n < p.N ? __ldg(p.w_scales + (int64_t)g * p.N + n) : 0x7f7f7f7fu;
-        }
-        const bool ok = mbar_wait_cluster(&sf_empty[u & 1], ((u >> 1) & 1) ^ 1, abort_flag, p.err);
+        for (int j = 0; j < 8; ++j)
+          w[j] = n0 + 32 * j < p.N ? __ldg(p.w_scales + (int64_t)g * p.N + n0 + 32 * j)
+                                   : 0x7f7f7f7fu;
+        const bool ok = mbar_wait_cluster(&sf_empty[b], ph, abort_flag, p.err);
         if (!__all_sync(0xffffffffu, ok)) {
           if (lane == 0) st_cluster_u32(peer_abort, 1);
           goto out;
         }
-        uint4* dst = reinterpret_cast<uint4*>(sSF + (u & 1) * Cfg::SF_BYTES);
+        ph ^= 1u;
+        uint4* dst = reinterpret_cast<uint4*>(sSF + b * Cfg::SF_BYTES);
         dst[lane] = make_uint4(a[0], a[1], a[2], a[3]);
         dst[32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
         dst[64 + lane] = make_uint4(w[4], w[5], w[6], w[7]);
         fence_proxy_async_shared();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(sf_full_lead + (u & 1) * 8);
+        if (lane == 0) mbar_arrive_cluster(sf_full_lead);
       }
     }
   } else {
     // Epilogue: TMEM lanes of `quarter`, the columns of `half` from the end that may
     // overlap the other accumulator (columns 232.. of the first, 0..23 of the second).
     constexpr int COLS = BN / 2;
-    const int quarter = warp & 3, half = (warp - 3) >> 2;
-    uint8_t* box = sBox + (warp - 3) * Cfg::BOX_BYTES;
-    float* bias = reinterpret_cast<float*>(sBias + (warp - 3) * Cfg::BIAS_BYTES);
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    uint8_t* box = sBox + (warp - 4) * Cfg::BOX_BYTES;
+    float* bias = reinterpret_cast<float*>(sBias + (warp - 4) * Cfg::BIAS_BYTES);
     const uint32_t tempty_lead = cluster_addr(tempty, 0);
     // a tile's bias is read while the tile before is finished
     float next_bias[COLS / 32];
