@@ -322,6 +322,7 @@ constexpr int held_ctas(int G, int V) {       // of an SM: registers for V vecto
 template <int G, int V, bool WIDE, bool E4M3>
 __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(const EdgeDesc d) {
   __shared__ __align__(16) float red[4][8];
+  if (E4M3) grid_dependents_may_start();   // the product that follows waits itself
   RowSum<G> sum{red};
   constexpr int ROWS = G == 32 ? held_threads(G) / 32 : 1;
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
@@ -386,6 +387,7 @@ __global__ void __launch_bounds__(G, row_ctas(G, V)) edge_row(const EdgeDesc d) 
   __shared__ __align__(16) float red[4][8];
   __shared__ uint64_t full;
   __shared__ int abort_flag;
+  if (E4M3) grid_dependents_may_start();
   RowSum<G> sum{red};
   const Columns<G, true> col;
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;

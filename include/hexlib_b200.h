@@ -379,7 +379,10 @@ HEXLIB_B200_API int hexlib_b200_attention_fp16(const void *q, const void *k, con
  * kernels above (no counterpart in the reference, whose weights are q4_0 and
  * whose only rotation is rope_2d). All of them take an empty batch (no rows, no
  * tokens) and then launch nothing, are ordered on `stream`, allocate nothing and
- * may be captured into a CUDA graph. `stream` must belong to the current device. */
+ * may be captured into a CUDA graph. `stream` must belong to the current device; like
+ * every per-kernel entry, the first call on a device sets the library up and must
+ * not be inside a capture. Rows, columns and K are at most 2^30. A bounded wait that
+ * expires is reported by hexlib_b200_stream_status. */
 
 /* THE E4M3 FORM of a matrix of R rows of K fp16 values. A row is cut into blocks
  * of 128 (the last one padded with zeros). A block's scale is the power of two
@@ -480,7 +483,7 @@ HEXLIB_B200_API int hexlib_b200_rope_pos_table(int scaling, int rot, double thet
  * projection are rotated in one call, in place when y is x and the strides are
  * equal. Elements from rot on are copied. positions is int32 [n_axes, T] (1 to 4
  * axes: text, or time, height and width), axis int32 [rot / 2] on the device,
- * clamped to [0, n_axes), NULL for axis 0 everywhere. Negative positions turn
+ * clamped to [0, n_axes), NULL for axis 0 everywhere; rot at most 24576. Negative positions turn
  * back: the call with negated positions is the gradient of the rotation and undoes
  * it (up to mscale^2). */
 HEXLIB_B200_API int hexlib_b200_rope_pos_fp16(const void *x, int64_t x_stride,

@@ -169,3 +169,14 @@ def test_empty_batches_need_nothing():
     assert rc("matmul_epilogue_e4m3", *with_(MM, M=0)) == OK
     assert rc("quantize_e4m3_fp16", *with_(QUANT, R=0)) == OK
     assert rc("rope_pos_fp16", *with_(ROPE, T=0)) == OK
+
+
+def test_more_than_the_largest_sizes_are_refused():
+    big = (1 << 30) + 1
+    for k in ("M", "K", "N"):
+        assert rc("matmul_epilogue_e4m3", *with_(MM, **{k: big})) == BAD
+    for k in ("R", "K"):
+        assert rc("quantize_e4m3_fp16", *with_(QUANT, **{k: big})) == BAD
+        assert rc("quantize_weight_e4m3_fp16", *with_(QUANT, **{k: big})) == BAD
+    for k in ("R", "C"):
+        assert rc("norm_gate_residual_fp16", *with_(EDGE, gate=None, rows=0, act=0, **{k: big})) == BAD
