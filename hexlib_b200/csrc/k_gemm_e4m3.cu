@@ -40,6 +40,13 @@ struct E4m3Params {
   int* err;
 };
 
+// The next 1024-byte boundary, reached by an offset: rounding the pointer as an integer
+// would lose that it is shared memory, and every access through it would be a generic
+// one, ordered with the stores of the output (16384 x 128 x 2304 with it: 27.5 us).
+__device__ __forceinline__ uint8_t* aligned_1024(uint8_t* p) {
+  return p + ((0u - smem_u32(p)) & 1023u);
+}
+
 __device__ __forceinline__ float finish(float v, int act) {
   if (act == 1) return gelu_tanh_f(v);
   if (act == 2) return gelu_erf_f(v);
@@ -82,8 +89,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int split = 1 << split_log2;
   using Cfg = TileCfg<BN>;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = aligned_1024(smem_raw);
   uint8_t* sW = smem;
   uint8_t* sA = smem + Cfg::STAGES * Cfg::W_BYTES;
   uint8_t* sSF = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
@@ -489,8 +495,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   using Cfg = PairCfg;
   constexpr int BN = Cfg::BN;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = aligned_1024(smem_raw);
   uint8_t* sA = smem;
   uint8_t* sW = smem + Cfg::STAGES * Cfg::A_BYTES;
   uint8_t* sBox = smem + Cfg::STAGES * Cfg::STAGE_BYTES;
