@@ -138,13 +138,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   if (split > 1) cluster_arrive();                   // waited for before the parts are sent
   grid_dependency_wait();
 
-  // The loops over blocks of K go round the ring of stages, whose addresses are then
-  // constants of the code: with addresses, descriptors and branches formed anew for
-  // each block by one lane, a block took 400 ns to issue, more than its loads.
+  // A role's whole warp runs its loop and an elected lane issues, which keeps addresses
+  // and descriptors in uniform registers: with one lane forming them anew a block took
+  // 400 ns to issue, more than its loads. The loops are not unrolled over the stages: the
+  // roles share the instruction cache (unrolled: 16384 x 768 x 2304 33.6 against 31.9 us on
+  // the pairs below; with the epilogue unrolled too 43).
   if (warp == 0) {
     int kb = kb0;
     for (uint32_t ph = 1; kb < kb1; ph ^= 1u) {
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < Cfg::STAGES; ++s) {
         if (kb >= kb1) break;
         if (!mbar_wait_warp(&empty[s], ph, abort_flag, p.err)) {
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     int kb = kb0;
     bool ok = true;
     for (uint32_t ph = 0; kb < kb1; ph ^= 1u) {
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < Cfg::STAGES; ++s) {
         if (kb >= kb1) break;
         const uint32_t b = u & 1, sf = tmem + BN + b * 8;
@@ -375,7 +377,9 @@ int launch_tile(const GemmE4m3Desc& g, int split_log2, int* err, cudaStream_t s)
 //
 // Epilogue: 8 warps, each 32 rows by 128 columns, 32 columns at a time: from tensor
 // memory through registers and a 2 KiB box in shared memory to rows of 64 bytes, stored
-// by the LSU at any alignment.
+// by the LSU at any alignment. One kernel for each activation, with and without a
+// residual: shorter code leaves the instruction cache to the other roles (16384 x 768 x
+// 2304 with GELU: 41.8 us as one kernel, 37.8 as six; without 32.0 and 31.6).
 constexpr int kPairThreads = 384;   // loads, MMAs, 2 warps of scales, 8 of epilogue
 
 struct PairCfg {
@@ -393,6 +397,7 @@ struct PairCfg {
 };
 
 // 32 columns of a row: bias (its 32 values in shared memory), activation.
+template <int ACT>
 __device__ __forceinline__ void activate32(const E4m3Params& p, const uint32_t (&r)[32],
                                            const float* bias, float2 (&v)[16]) {
 #pragma unroll
@@ -406,10 +411,10 @@ __device__ __forceinline__ void activate32(const E4m3Params& p, const uint32_t (
       v[j + 1] = __fadd2_rn(v[j + 1], make_float2(b.z, b.w));
     }
   }
-  if (p.act == 1) {
+  if (ACT == 1) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = gelu_tanh_f2(v[j]);
-  } else if (p.act == 2) {
+  } else if (ACT == 2) {
 #pragma unroll
     for (int j = 0; j < 16; ++j) v[j] = make_float2(gelu_erf_f(v[j].x), gelu_erf_f(v[j].y));
   }
@@ -489,6 +494,7 @@ struct TileWalk {
   }
 };
 
+template <int ACT, bool RESID>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_e4m3_pair(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                    const E4m3Params p) {
@@ -546,7 +552,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t full_lead = cluster_addr(full, 0);
     int kb = 0;
     for (uint32_t ph = 1; t.left; ph ^= 1u) {
-#pragma unroll
+#pragma unroll 1
       for (int s = 0; s < Cfg::STAGES; ++s) {
         if (!t.left) break;
         if (!mbar_wait_cluster_warp(&empty[s], ph, abort_flag, p.err)) {
@@ -575,7 +581,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       uint32_t u = 0, i = 0;                         // scale words, tiles so far
       int kb = 0;
       for (uint32_t ph = 0; t.left; ph ^= 1u) {
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < Cfg::STAGES; ++s) {
           if (!t.left) break;
           const uint32_t b = u & 1, sf = tmem + Cfg::SF + b * 12;
@@ -686,7 +692,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int j = 0; j < COLS / 32; ++j) bias[j * 32 + lane] = next_bias[j];
       __syncwarp();
       if (t.left) read_bias(t.n);
-      if (p.resid) box_load(p, box, row0, n0 + (half ? COLS - 32 : 0), lane);
+      if (RESID) box_load(p, box, row0, n0 + (half ? COLS - 32 : 0), lane);
       const bool ok = mbar_wait_cluster(&tfull[i & 1], (i >> 1) & 1, abort_flag, p.err);
       if (!__all_sync(0xffffffffu, ok)) {
         if (lane == 0) st_cluster_u32(peer_abort, 1);
@@ -707,15 +713,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (lane == 0) mbar_arrive_cluster_relaxed(tempty_lead);
         }
         float2 v[16];
-        activate32(p, r, bias + c, v);
-        if (p.resid) {
+        activate32<ACT>(p, r, bias + c, v);
+        if (RESID) {
           if (j > 0) box_load(p, box, row0, n0 + c, lane);
           __syncwarp();
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint4* slot = reinterpret_cast<uint4*>(box + box_at(lane, q));
-          if (p.resid) {
+          if (RESID) {
             const uint4 u = *slot;
             const uint32_t h[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -745,6 +751,15 @@ out:
   }
 }
 
+using PairKernel = void (*)(CUtensorMap, CUtensorMap, E4m3Params);
+PairKernel pair_kernel(int act, bool resid) {
+  if (resid)
+    return act == 0 ? gemm_e4m3_pair<0, true>
+                    : act == 1 ? gemm_e4m3_pair<1, true> : gemm_e4m3_pair<2, true>;
+  return act == 0 ? gemm_e4m3_pair<0, false>
+                  : act == 1 ? gemm_e4m3_pair<1, false> : gemm_e4m3_pair<2, false>;
+}
+
 std::atomic<int> g_pairs{0};   // pairs resident at once, 0 until the kernel is loaded
 
 int launch_pair(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
@@ -771,7 +786,7 @@ int launch_pair(const GemmE4m3Desc& g, int* err, cudaStream_t s) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, gemm_e4m3_pair, ta, tw, p) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, pair_kernel(g.act, g.resid != nullptr), ta, tw, p) != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;
   }
@@ -787,10 +802,14 @@ bool load_pair() {
   cfg.attrs = cluster_of(attr, 2);
   cfg.numAttrs = 1;
   int pairs = 0;
-  if (cudaFuncSetAttribute(gemm_e4m3_pair, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           PairCfg::SMEM_BYTES) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&pairs, gemm_e4m3_pair, &cfg) != cudaSuccess)
-    return false;
+  for (int act = 0; act < 3; ++act)
+    for (int resid = 0; resid < 2; ++resid)
+      if (cudaFuncSetAttribute((const void*)pair_kernel(act, resid != 0),
+                               cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               PairCfg::SMEM_BYTES) != cudaSuccess ||
+          cudaOccupancyMaxActiveClusters(&pairs, (const void*)pair_kernel(act, resid != 0),
+                                         &cfg) != cudaSuccess)
+        return false;
   g_pairs.store(pairs, std::memory_order_relaxed);
   return pairs > 0;
 }
