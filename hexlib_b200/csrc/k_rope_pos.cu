@@ -21,6 +21,7 @@ struct RopeShape {
   int tokens;      // of a CTA
   int pairs;       // rot / 2
   int rot_items;   // items of a head that rotate, then those that are copied
+  int copy_w;      // elements of a copied item (8, 4 or 2; 1 where nothing is a vector)
   int items;       // of a head, of them the ones to do (in place nothing is copied)
   int head_split;  // CTAs that share a token tile's heads
   int heads;       // of a CTA
@@ -54,15 +55,38 @@ __device__ __forceinline__ void tile_phases(const RopePosDesc& d, const RopeShap
   }
 }
 
-// Rows of whole 16-byte vectors: an item is 16 elements of a head (half layout, 8 pairs)
-// or 8 (interleaved, 4 pairs; or copied). Bound by memory; a thread has two items in
+// Rows of whole vectors of W = 8, 4 or 2 elements: an item is W elements of either half
+// of a head (half layout, W pairs), W elements (interleaved, W / 2 pairs), or one vector
+// copied, as wide as its rows allow.
+// Bound by memory; a thread has two items in
 // flight, the first two from before the phases are formed, which hides the positions'
 // way through memory behind the rows' (32768 tokens of 40 of 48 heads of 128: 112 us,
 // 5.97 TB/s; 135 without, 118 with four items in flight and half the warps; 4097 tokens
-// of 24 heads of 64, three axes: 8.0 us, of which 3.8 are memory's).
+// of 24 heads of 64, three axes: 8.0 us, of which 3.8 are memory's; 32768 of 40 heads of 96,
+// 24 rotated by halves: 101 us on vectors of 4 and copies of 8, 145 with copies of 4, over
+// 250 pair by pair).
 constexpr int kBatch = 2;
 
-template <bool INTERLEAVED>
+template <int W>
+__device__ __forceinline__ void load_words(uint32_t (&w)[W / 2], const __half* p) {
+  if constexpr (W == 8) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  } else if constexpr (W == 4) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    w[0] = u.x; w[1] = u.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+template <int W>
+__device__ __forceinline__ void store_words(__half* p, const uint32_t (&w)[W / 2]) {
+  if constexpr (W == 8) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+  else if constexpr (W == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+
+template <int W, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rope_pos_vec(const RopePosDesc d, const RopeShape sh) {
   extern __shared__ float2 cs[];                       // [tokens][pairs]
   constexpr int VECS = INTERLEAVED ? 1 : 2;            // of a rotating item
@@ -84,9 +108,9 @@ __global__ void __launch_bounds__(kThreads) rope_pos_vec(const RopePosDesc d, co
     return Item{(int)t, i < total && h < heads ? h : -1, (int)(i - th * sh.items)};
   };
   auto first_of = [&](const Item& m) {                 // its first element within the head
-    return m.item < sh.rot_items ? m.item * 8 : d.rot + (m.item - sh.rot_items) * 8;
+    return m.item < sh.rot_items ? m.item * W : d.rot + (m.item - sh.rot_items) * sh.copy_w;
   };
-  uint4 u[kBatch][VECS];
+  uint32_t u[kBatch][VECS][W / 2], v[kBatch][4];      // (v: copied, where wider than W)
   auto load = [&](uint32_t i0) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
@@ -94,13 +118,18 @@ __global__ void __launch_bounds__(kThreads) rope_pos_vec(const RopePosDesc d, co
       if (m.h < 0) continue;
       const __half* x = (const __half*)d.x + (t0 + m.t) * d.x_stride + (int64_t)(h0 + m.h) * d.D +
                         first_of(m);
-      u[b][0] = *reinterpret_cast<const uint4*>(x);
-      if (!INTERLEAVED && m.item < sh.rot_items)
-        u[b][VECS - 1] = *reinterpret_cast<const uint4*>(x + half);
+      if (W < 8 && m.item >= sh.rot_items) {
+        if (sh.copy_w == 8) load_words<8>(v[b], x);
+        else if (sh.copy_w == 4) load_words<4>(reinterpret_cast<uint32_t(&)[2]>(v[b]), x);
+        else load_words<2>(reinterpret_cast<uint32_t(&)[1]>(v[b]), x);
+        continue;
+      }
+      load_words<W>(u[b][0], x);
+      if (!INTERLEAVED && m.item < sh.rot_items) load_words<W>(u[b][VECS - 1], x + half);
     }
   };
   load(threadIdx.x);
-  tile_phases<INTERLEAVED ? 4 : 8>(d, sh, t0, tokens, cs);
+  tile_phases<INTERLEAVED ? W / 2 : W>(d, sh, t0, tokens, cs);
   __syncthreads();
   for (uint32_t i0 = threadIdx.x; i0 < total; i0 += kBatch * kThreads) {
 #pragma unroll
@@ -110,27 +139,32 @@ __global__ void __launch_bounds__(kThreads) rope_pos_vec(const RopePosDesc d, co
       __half* y = (__half*)d.y + (t0 + m.t) * d.y_stride + (int64_t)(h0 + m.h) * d.D + first_of(m);
       if (m.item < sh.rot_items) {
         const float2* c = cs + m.t * sh.pairs + m.item;
-        uint32_t a[4] = {u[b][0].x, u[b][0].y, u[b][0].z, u[b][0].w};
+        uint32_t(&a)[W / 2] = u[b][0];
         if constexpr (INTERLEAVED) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < W / 2; ++q) {
             const float2 f = halves(a[q]), k = c[q * sh.rot_items];
             a[q] = pack(f.x * k.x - f.y * k.y, f.x * k.y + f.y * k.x);
           }
         } else {
-          uint32_t e[4] = {u[b][VECS - 1].x, u[b][VECS - 1].y, u[b][VECS - 1].z, u[b][VECS - 1].w};
+          uint32_t(&e)[W / 2] = u[b][VECS - 1];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < W / 2; ++q) {
             const float2 fa = halves(a[q]), fb = halves(e[q]);
             const float2 k0 = c[2 * q * sh.rot_items], k1 = c[(2 * q + 1) * sh.rot_items];
             a[q] = pack(fa.x * k0.x - fb.x * k0.y, fa.y * k1.x - fb.y * k1.y);
             e[q] = pack(fa.x * k0.y + fb.x * k0.x, fa.y * k1.y + fb.y * k1.x);
           }
-          *reinterpret_cast<uint4*>(y + half) = make_uint4(e[0], e[1], e[2], e[3]);
+          store_words<W>(y + half, e);
         }
-        u[b][0] = make_uint4(a[0], a[1], a[2], a[3]);
       }
-      *reinterpret_cast<uint4*>(y) = u[b][0];
+      if (W < 8 && m.item >= sh.rot_items) {
+        if (sh.copy_w == 8) store_words<8>(y, v[b]);
+        else if (sh.copy_w == 4) store_words<4>(y, reinterpret_cast<uint32_t(&)[2]>(v[b]));
+        else store_words<2>(y, reinterpret_cast<uint32_t(&)[1]>(v[b]));
+        continue;
+      }
+      store_words<W>(y, u[b][0]);
     }
     load(i0 + kBatch * kThreads);
   }
@@ -173,7 +207,9 @@ constexpr int kMaxPairBytes = 96 * 1024;   // cosines and sines of a tile
 }  // namespace
 
 int rope_pos_kernels_init() {
-  for (auto k : {rope_pos_vec<true>, rope_pos_vec<false>, rope_pos_any<true>, rope_pos_any<false>})
+  for (auto k : {rope_pos_vec<8, true>, rope_pos_vec<8, false>, rope_pos_vec<4, true>,
+                 rope_pos_vec<4, false>, rope_pos_vec<2, true>, rope_pos_vec<2, false>,
+                 rope_pos_any<true>, rope_pos_any<false>})
     if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxPairBytes) !=
         cudaSuccess) {
       cudaGetLastError();
@@ -189,12 +225,20 @@ int launch_rope_pos(const RopePosDesc& desc, cudaStream_t s) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.y) |
                          static_cast<uintptr_t>(2 * d.x_stride) |
                          static_cast<uintptr_t>(2 * d.y_stride) | static_cast<uintptr_t>(2 * d.D);
-  const bool vec = bits % 16 == 0 && d.rot % (inter ? 8 : 16) == 0 && d.D <= 4096;
+  // the widest vector that divides the rows and the rotated part (each half of it)
+  const int part = inter ? d.rot : d.rot / 2;
+  int w = 8;
+  while (w > 1 && (bits % (2 * w) != 0 || part % w != 0)) w /= 2;
+  if (d.D > 4096) w = 1;
   RopeShape sh;
   sh.pairs = d.rot / 2;
   if ((int64_t)sh.pairs * 8 > kMaxPairBytes) return HEXLIB_B200_ERR_INVAL_PARAMS;
-  sh.rot_items = vec ? sh.pairs / (inter ? 4 : 8) : sh.pairs;
-  sh.items = sh.rot_items + (d.x == d.y ? 0 : vec ? (d.D - d.rot) / 8 : d.D - d.rot);
+  sh.rot_items = w > 1 ? part / w : sh.pairs;
+  sh.copy_w = w;                           // (w divides rot, D and the strides)
+  while (w > 1 && sh.copy_w < 8 &&
+         ((bits | static_cast<uintptr_t>(2 * d.rot)) % (4 * sh.copy_w)) == 0)
+    sh.copy_w *= 2;
+  sh.items = sh.rot_items + (d.x == d.y ? 0 : (d.D - d.rot) / sh.copy_w);
   // tokens of a CTA: a few cosines and about eight items to a thread, but four CTAs to
   // an SM where there are tokens for them; few tokens split their heads over CTAs
   const int64_t per_token = (int64_t)d.H * sh.items;
@@ -217,8 +261,12 @@ int launch_rope_pos(const RopePosDesc& desc, cudaStream_t s) {
   const unsigned grid = (unsigned)(tiles * sh.head_split);
   const size_t smem = (size_t)sh.tokens * sh.pairs * sizeof(float2);
   auto go = [&](auto kernel) { kernel<<<grid, kThreads, smem, s>>>(d, sh); };
-  if (vec) inter ? go(rope_pos_vec<true>) : go(rope_pos_vec<false>);
-  else inter ? go(rope_pos_any<true>) : go(rope_pos_any<false>);
+  switch (w) {
+    case 8: inter ? go(rope_pos_vec<8, true>) : go(rope_pos_vec<8, false>); break;
+    case 4: inter ? go(rope_pos_vec<4, true>) : go(rope_pos_vec<4, false>); break;
+    case 2: inter ? go(rope_pos_vec<2, true>) : go(rope_pos_vec<2, false>); break;
+    default: inter ? go(rope_pos_any<true>) : go(rope_pos_any<false>);
+  }
   if (cudaPeekAtLastError() != cudaSuccess) {
     cudaGetLastError();
     return HEXLIB_B200_ERR_CUDA;

@@ -31,7 +31,9 @@ def rotate(x, pos, table, axis, mscale, H, D, rot, layout, y=None, y_stride=None
 @pytest.mark.parametrize("T,H,D,rot", [(1, 1, 2, 2), (1, 4, 128, 128), (3, 2, 64, 32), (5, 7, 80, 20), (2, 3, 10, 6),
                                        (9, 1, 256, 256), (33, 12, 64, 64), (8, 20, 128, 32), (17, 5, 96, 96), (4, 2, 33, 2),
                                        (130, 3, 192, 48), (2, 64, 128, 64),
-                                       (3, 1, 16, 16), (700, 1, 16, 16), (1300, 2, 32, 16), (900, 1, 8, 8), (2, 1500, 16, 16)])
+                                       (3, 1, 16, 16), (700, 1, 16, 16), (1300, 2, 32, 16), (900, 1, 8, 8), (2, 1500, 16, 16),
+                                       (40, 5, 96, 24), (41, 3, 80, 40), (700, 2, 32, 8), (25, 4, 36, 12), (19, 3, 22, 10),
+                                       (650, 1, 20, 20), (11, 2, 4100, 64)])
 def test_layouts_and_partial_heads(T, H, D, rot, layout):
     rng = np.random.default_rng(T + H + D + rot)
     x = rng.standard_normal((T, H * D)).astype(np.float16)
@@ -89,7 +91,7 @@ def test_axes_and_clamped_axis_numbers(A):
 
 
 @pytest.mark.parametrize("layout", [0, 1])
-@pytest.mark.parametrize("H,HV,D,rot", [(6, 2, 64, 64), (3, 1, 80, 40), (5, 2, 34, 6), (8, 4, 128, 32)])
+@pytest.mark.parametrize("H,HV,D,rot", [(6, 2, 64, 64), (3, 1, 80, 40), (5, 2, 34, 6), (8, 4, 128, 32), (4, 2, 96, 24), (7, 1, 20, 4)])
 def test_packed_projection_in_place_and_out_of_place(H, HV, D, rot, layout):
     T = 21
     rng = np.random.default_rng(D)
