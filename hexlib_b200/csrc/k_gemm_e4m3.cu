@@ -428,7 +428,8 @@ __device__ __forceinline__ uint32_t box_at(int r, int q) {
 }
 
 // The box between shared and global memory, rows [row0, row0 + 32) clipped to M and
-// columns [n, n + 32) to N: 16 bytes to a lane where the rows allow it, else 2.
+// columns [n, n + 32) to N: 16 bytes to a lane where all rows allow it, else two values,
+// as one word where the row allows it (with an odd N every other row does).
 __device__ __forceinline__ void box_store(const E4m3Params& p, const uint8_t* box, int64_t row0,
                                           int n, int lane) {
   if (p.wide) {
@@ -440,11 +441,20 @@ __device__ __forceinline__ void box_store(const E4m3Params& p, const uint8_t* bo
             *reinterpret_cast<const uint4*>(box + box_at(r, q));
     }
   } else {
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-      if (row0 + r < p.M && n + lane < p.N)
-        p.out[(row0 + r) * p.N + n + lane] =
-            *reinterpret_cast<const __half*>(box + box_at(r, lane >> 3) + (lane & 7) * 2);
+    const int k = lane & 15, left = p.N - n - 2 * k;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const int r = i * 2 + (lane >> 4);
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(box + box_at(r, k >> 2) + (k & 3) * 4);
+      if (row0 + r >= p.M || left <= 0) continue;
+      __half* to = p.out + (row0 + r) * p.N + n + 2 * k;
+      if (left > 1 && (reinterpret_cast<uintptr_t>(to) & 3u) == 0) {
+        *reinterpret_cast<uint32_t*>(to) = w;
+      } else {
+        to[0] = __ushort_as_half((unsigned short)w);
+        if (left > 1) to[1] = __ushort_as_half((unsigned short)(w >> 16));
+      }
+    }
   }
 }
 __device__ __forceinline__ void box_load(const E4m3Params& p, uint8_t* box, int64_t row0, int n,
@@ -462,10 +472,26 @@ __device__ __forceinline__ void box_load(const E4m3Params& p, uint8_t* box, int6
     for (int i = 0; i < 4; ++i)
       *reinterpret_cast<uint4*>(box + box_at(i * 8 + (lane >> 2), lane & 3)) = u[i];
   } else {
-#pragma unroll 8
-    for (int r = 0; r < 32; ++r)
-      *reinterpret_cast<__half*>(box + box_at(r, lane >> 3) + (lane & 7) * 2) =
-          row0 + r < p.M && n + lane < p.N ? p.resid[(row0 + r) * p.N + n + lane] : __half(0.f);
+    // eight rows' loads at once, a value each, so that none waits for a branch
+    const int k = lane & 15, left = p.N - n - 2 * k;
+#pragma unroll
+    for (int i0 = 0; i0 < 16; i0 += 4) {
+      unsigned short lo[4], hi[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = (i0 + i) * 2 + (lane >> 4);
+        const unsigned short* from = reinterpret_cast<const unsigned short*>(p.resid) +
+                                     (row0 + r) * p.N + n + 2 * k;
+        lo[i] = row0 + r < p.M && left > 0 ? from[0] : 0;
+        hi[i] = row0 + r < p.M && left > 1 ? from[1] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = (i0 + i) * 2 + (lane >> 4);
+        *reinterpret_cast<uint32_t*>(box + box_at(r, k >> 2) + (k & 3) * 4) =
+            lo[i] | ((uint32_t)hi[i] << 16);
+      }
+    }
   }
 }
 
