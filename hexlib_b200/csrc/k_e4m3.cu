@@ -18,7 +18,8 @@ int grid_for(int64_t items) {
 
 // Half a warp per scale word: 512 values of a row, a block of 128 at a time, 8 to a
 // lane, so a lane has four 16-byte loads in flight and a word is stored whole. Bound
-// by memory: 2 bytes read and 1 written per value.
+// by memory: 2 bytes read and 1 written per value (8192 x 4096: 18.7 us, 5.4 TB/s;
+// 60.6 us a block to a warp and a value at a time).
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) quantize_e4m3(const __half* __restrict__ x,
                                                           uint8_t* __restrict__ codes,

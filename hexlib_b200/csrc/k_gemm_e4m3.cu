@@ -42,7 +42,7 @@ struct E4m3Params {
 
 // The next 1024-byte boundary, reached by an offset: rounding the pointer as an integer
 // would lose that it is shared memory, and every access through it would be a generic
-// one, ordered with the stores of the output (16384 x 128 x 2304 with it: 27.5 us).
+// one, ordered with the stores of the output (16384 x 128 x 2304: 27.5 us then, 24.9 so).
 __device__ __forceinline__ uint8_t* aligned_1024(uint8_t* p) {
   return p + ((0u - smem_u32(p)) & 1023u);
 }
@@ -859,8 +859,8 @@ int gemm_e4m3_kernels_init() {
 // The kernel and tiling with the least estimated time, in us. The estimate is a fixed
 // cost, the blocks of K a CTA goes through at the rate measured for one or two CTAs on an
 // SM (68 and 108 bytes a ns), its epilogue, and the joining of a split; w from memory at
-// 6 TB/s bounds the loop below. It was fitted to sweeps of every choice: 4096 x 4096 for 1 token 8.5 us on
-// 16-token tiles split by 4 (16.9 unsplit), for 256 tokens 16.0 on 64-token tiles (22.0 on
+// 6 TB/s bounds the loop below. It was fitted to sweeps of every choice: 4096 x 4096 for
+// 1 token 8.5 us on 16-token tiles split by 4 (16.9 unsplit), for 256 tokens 16.0 on 64-token tiles (22.0 on
 // pairs, 27 split); 1000 x 1000 for 2000 tokens 10.2 on pairs and on 64-token tiles,
 // 2304 x 256 for 4096 tokens 11.4 on pairs.
 struct Choice {
