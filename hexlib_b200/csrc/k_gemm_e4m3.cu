@@ -860,9 +860,9 @@ int gemm_e4m3_kernels_init() {
 // cost, the blocks of K a CTA goes through at the rate measured for one or two CTAs on an
 // SM (68 and 108 bytes a ns), its epilogue, and the joining of a split; w from memory at
 // 6 TB/s bounds the loop below. It was fitted to sweeps of every choice: 4096 x 4096 for
-// 1 token 8.5 us on 16-token tiles split by 4 (16.9 unsplit), for 256 tokens 16.0 on 64-token tiles (22.0 on
-// pairs, 27 split); 1000 x 1000 for 2000 tokens 10.2 on pairs and on 64-token tiles,
-// 2304 x 256 for 4096 tokens 11.4 on pairs.
+// 1 token 8.5 us on 16-token tiles split by 4 (16.9 unsplit), for 256 tokens 16.0 on
+// 64-token tiles (22.0 on pairs, 27 split); 1000 x 1000 for 2000 tokens 10.2 on pairs and
+// on 64-token tiles, 2304 x 256 for 4096 tokens 11.4 on pairs.
 struct Choice {
   int bn, split_log2;                      // bn = 0: CTA pairs
 };
