@@ -713,6 +713,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int n0 = t.n * BN + half * COLS;
       t.next();
       const bool overlaps = half != (int)(i & 1);    // this half has the overlap
+      tc_fence_before();                             // (the loads of the tile before)
       if (!overlaps && lane == 0) mbar_arrive_cluster_relaxed(tempty_lead);
 #pragma unroll
       for (int j = 0; j < COLS / 32; ++j) bias[j * 32 + lane] = next_bias[j];

@@ -264,3 +264,71 @@ def test_product_of_many_tiles(M, K, N, act, with_bias, with_resid):
     if not with_resid:
         product(a, w, M, K, N, act, bias, None, out=y)
         assert np.array_equal(first, U.host(y))
+
+
+@pytest.mark.parametrize("M,K,N", [(3, 2048, 640), (200, 1024, 512), (2600, 640, 1032)])
+def test_product_after_copies_events_and_forks(M, K, N):
+    # what may stand before a product in a stream: a copy, a fill, a wait for another
+    # stream, another product; eager, and as nodes of one captured graph
+    import torch
+    rng = np.random.default_rng(M)
+    a, w = operands(rng, M, K, N)
+    want = U.host(product(a, w, M, K, N))
+    x = U.dev(rng.standard_normal((M, K)).astype(np.float16))
+    xq, xs = quantize(x)
+    want2 = U.host(product((xq, xs), w, M, K, N))
+    src, scales = a[0].clone(), a[1].clone()
+    q, s = torch.zeros_like(src), torch.zeros_like(scales)
+    q2, s2 = torch.zeros_like(xq), torch.zeros_like(xs)
+    y, y2 = (torch.empty((M, N), dtype=torch.float16, device="cuda") for _ in range(2))
+    fork = torch.cuda.Stream()
+
+    def go():
+        main = torch.cuda.current_stream()
+        y.fill_(-1)
+        q.copy_(src)
+        fork.wait_stream(main)
+        with torch.cuda.stream(fork):
+            s.copy_(scales)
+            U.call("hexlib_b200_quantize_e4m3_fp16", U.ptr(x), U.ptr(q2), U.ptr(s2), M, K, fork.cuda_stream)
+            product((q2, s2), w, M, K, N, out=y2) if not torch.cuda.is_current_stream_capturing() else U.call(
+                "hexlib_b200_matmul_epilogue_e4m3", U.ptr(q2), U.ptr(s2), U.ptr(w[0]), U.ptr(w[1]), None, U.ptr(y2), M, K, N, 0,
+                fork.cuda_stream)
+        main.wait_stream(fork)
+        for _ in range(2):
+            U.call("hexlib_b200_matmul_epilogue_e4m3", U.ptr(q), U.ptr(s), U.ptr(w[0]), U.ptr(w[1]), None, U.ptr(y), M, K, N, 0,
+                   main.cuda_stream)
+
+    def check():
+        torch.cuda.synchronize()
+        assert np.array_equal(U.host(y), want) and np.array_equal(U.host(y2), want2)
+        for t in (q, s, q2, s2):
+            t.zero_()
+        y.zero_(), y2.zero_()
+        torch.cuda.synchronize()
+    go()
+    check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go()
+    for _ in range(3):
+        graph.replay()
+        check()
+
+
+def test_a_weight_quantized_just_before_its_product():
+    import torch
+    rng = np.random.default_rng(8)
+    for M, K, N in ((1, 4096, 2048), (300, 512, 768)):
+        a, _ = operands(rng, M, K, 8)
+        ws = [(rng.standard_normal((K, N)) / K ** 0.5).astype(np.float16) for _ in range(2)]
+        dev = [U.dev(w) for w in ws]
+        q, s = u8((N, B.pitch(K))), u8((B.groups(K), N, 4))
+        ys = [torch.empty((M, N), dtype=torch.float16, device="cuda") for _ in range(6)]
+        for i, y in enumerate(ys):
+            U.call("hexlib_b200_quantize_weight_e4m3_fp16", U.ptr(dev[i % 2]), U.ptr(q), U.ptr(s), K, N, U.stream())
+            U.call("hexlib_b200_matmul_epilogue_e4m3", U.ptr(a[0]), U.ptr(a[1]), U.ptr(q), U.ptr(s), None, U.ptr(y), M, K, N,
+                   0, U.stream())
+        for i, y in enumerate(ys):
+            ref, bound = B.product(a[2], B.values(*B.quantize(np.ascontiguousarray(ws[i % 2].T))), None, None, 0)
+            B.assert_within(U.host(y), ref, bound, f"call {i}")

@@ -100,7 +100,7 @@ def test_without_gate_or_block_output_or_next_norm(C):
     check(dict(c, pre_b=None, post_b=None), layer=True)
 
 
-@pytest.mark.parametrize("C", [768, 1203, 4096])
+@pytest.mark.parametrize("C", [768, 1203, 2048, 4096, 17000])
 @pytest.mark.parametrize("in_place", ["x", "y", "h"])
 def test_in_place(in_place, C):
     c = case(70, C, False, True, 70)
