@@ -472,13 +472,14 @@ __device__ __forceinline__ void box_load(const E4m3Params& p, uint8_t* box, int6
     for (int i = 0; i < 4; ++i)
       *reinterpret_cast<uint4*>(box + box_at(i * 8 + (lane >> 2), lane & 3)) = u[i];
   } else {
-    // eight rows' loads at once, a value each, so that none waits for a branch
+    // sixteen rows' loads at once, a value each, so that none waits for a branch (4750 x 260
+    // x 6795 with the residual: 129 us with eight rows, 124 with sixteen)
     const int k = lane & 15, left = p.N - n - 2 * k;
 #pragma unroll
-    for (int i0 = 0; i0 < 16; i0 += 4) {
-      unsigned short lo[4], hi[4];
+    for (int i0 = 0; i0 < 16; i0 += 8) {
+      unsigned short lo[8], hi[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const int r = (i0 + i) * 2 + (lane >> 4);
         const unsigned short* from = reinterpret_cast<const unsigned short*>(p.resid) +
                                      (row0 + r) * p.N + n + 2 * k;
@@ -486,7 +487,7 @@ __device__ __forceinline__ void box_load(const E4m3Params& p, uint8_t* box, int6
         hi[i] = row0 + r < p.M && left > 1 ? from[1] : 0;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const int r = (i0 + i) * 2 + (lane >> 4);
         *reinterpret_cast<uint32_t*>(box + box_at(r, k >> 2) + (k & 3) * 4) =
             lo[i] | ((uint32_t)hi[i] << 16);
