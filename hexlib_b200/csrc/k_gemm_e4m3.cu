@@ -364,7 +364,10 @@ int launch_tile(const GemmE4m3Desc& g, int split_log2, int* err, cudaStream_t s)
 // [232, 488), and the scales take [488, 512). The epilogue reads the overlap first and
 // tells the MMA thread as soon as it has; the next tile's MMAs start then, while the
 // rest of the tile is finished. That arrival also says that the warp is done with
-// every earlier tile, so one barrier covers both uses. (Tiles of 192 columns with two
+// every earlier tile, so one arrival covers both uses. A warp may arrive for the next tile
+// before another has for this one -- the half without the overlap arrives as it begins
+// the tile -- so tiles take turns at two barriers; further ahead no warp comes, since it
+// waits for its tile's accumulator in between. (Tiles of 192 columns with two
 // whole accumulators: 16384 x 768 x 2304 in 42.5 us against 37.6, 8192 x 4096 x 4096 in
 // 134 against 108; narrower MMAs re-read the tokens' rows more often.)
 //
@@ -373,7 +376,8 @@ int launch_tile(const GemmE4m3Desc& g, int split_log2, int* err, cudaStream_t s)
 //   sf_full[b]  leader: both CTAs have written scale buffer b
 //   sf_empty[b] both: the MMAs that use scale buffer b are done
 //   tfull[a]    both: accumulator a is complete
-//   tempty      leader: the pair's 16 epilogue warps have read the overlap
+//   tempty[a]   leader: the pair's 16 epilogue warps have read accumulator a's overlap
+//               and the whole of the other
 //
 // Epilogue: 8 warps, each 32 rows by 128 columns, 32 columns at a time: from tensor
 // memory through registers and a 2 KiB box in shared memory to rows of 64 bytes, stored
@@ -540,7 +544,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint64_t* sf_empty = sf_full + 2;
   uint64_t* tfull = sf_empty + 2;
   uint64_t* tempty = tfull + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -554,8 +558,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       mbar_init(&sf_full[b], 2);
       mbar_init(&sf_empty[b], 1);
       mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 16);
     }
-    mbar_init(tempty, 16);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmA);
@@ -616,7 +620,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           const bool fresh = (kb & 3) == 0;
           bool ok = true;
           if (kb == 0 && i > 0)
-            ok = mbar_wait_cluster_warp(tempty, (i - 1) & 1, abort_flag, p.err);
+            ok = mbar_wait_cluster_warp(&tempty[(i - 1) & 1], ((i - 1) >> 1) & 1, abort_flag,
+                                        p.err);
           if (fresh)
             ok = ok && mbar_wait_cluster_warp(&sf_full[b], (u >> 1) & 1, abort_flag, p.err);
           ok = ok && mbar_wait_cluster_warp(&full[s], ph, abort_flag, p.err);
@@ -715,7 +720,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       t.next();
       const bool overlaps = half != (int)(i & 1);    // this half has the overlap
       tc_fence_before();                             // (the loads of the tile before)
-      if (!overlaps && lane == 0) mbar_arrive_cluster_relaxed(tempty_lead);
+      if (!overlaps && lane == 0) mbar_arrive_cluster_relaxed(tempty_lead + (i & 1) * 8);
 #pragma unroll
       for (int j = 0; j < COLS / 32; ++j) bias[j * 32 + lane] = next_bias[j];
       __syncwarp();
@@ -738,7 +743,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (overlaps && j == 0) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster_relaxed(tempty_lead);
+          if (lane == 0) mbar_arrive_cluster_relaxed(tempty_lead + (i & 1) * 8);
         }
         float2 v[16];
         activate32<ACT>(p, r, bias + c, v);

@@ -332,3 +332,41 @@ def test_a_weight_quantized_just_before_its_product():
         for i, y in enumerate(ys):
             ref, bound = B.product(a[2], B.values(*B.quantize(np.ascontiguousarray(ws[i % 2].T))), None, None, 0)
             B.assert_within(U.host(y), ref, bound, f"call {i}")
+
+
+@pytest.mark.parametrize("M,K,N,in_place", [(2600, 300, 1001, False), (2600, 300, 1001, True), (9500, 130, 770, False),
+                                            (9500, 130, 770, True), (2600, 300, 1032, True), (2600, 300, 259, False)])
+def test_residual_from_any_element_reads_only_its_own(M, K, N, in_place):
+    import torch
+    rng = np.random.default_rng(M + N)
+    a, w = operands(rng, M, K, N)
+    resid = rng.standard_normal((M, N)).astype(np.float16)
+    ref, bound = B.product(a[2], w[2], None, resid, 1)
+    first = None
+    for shift in (0, 1, 2, 3, 8):
+        flat = torch.full((64 + shift + M * N + 64,), float("nan"), dtype=torch.float16, device="cuda")
+        view = flat[64 + shift:64 + shift + M * N]
+        view.copy_(U.dev(resid).reshape(-1))
+        y = product(a, w, M, K, N, 1, None, view, out=view if in_place else None)
+        y = U.host(y).reshape(M, N)
+        if first is None:
+            first = y
+            B.assert_within(y, ref, bound, "aligned")
+        assert np.array_equal(first, y), shift
+        assert bool(flat[:64 + shift].isnan().all()) and bool(flat[64 + shift + M * N:].isnan().all())
+
+
+def test_residual_and_output_larger_than_l2():
+    M, K, N = 4750, 260, 6800
+    rng = np.random.default_rng(5)
+    a, w = operands(rng, M, K, N)
+    r = U.dev(rng.standard_normal((M, N)).astype(np.float16))
+    whole = product(a, w, M, K, N, 0, None, r)
+    half = M // 2
+    s = U.host(a[1]).reshape(-1, M, 4)
+    for lo, hi in ((0, half), (half, M)):
+        part = (a[0][lo:hi].contiguous(), U.dev(np.ascontiguousarray(s[:, lo:hi])), None)
+        y = product(part, w, hi - lo, K, N, 0, None, r[lo:hi].contiguous())
+        assert bool((y == whole[lo:hi]).all())
+    ref, bound = B.product(a[2][-300:], w[2], None, U.host(r)[-300:], 0)
+    B.assert_within(U.host(whole)[-300:], ref, bound, "last rows")
