@@ -37,6 +37,7 @@ struct E4m3Params {
   int M, N, num_kb, act;
   int tiles_n;                // tiles along N
   int wide;                   // rows of out and resid are whole 16-byte vectors
+  int ahead;                  // fetch the residual to L2 a tile ahead
   int* err;
 };
 
@@ -294,6 +295,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
+constexpr int64_t kFitsL2 = 120ll << 20;   // bytes: of 126 MB of L2
+
 E4m3Params params_of(const GemmE4m3Desc& g, int* err) {
   E4m3Params p = {};
   p.a_scales = g.a_scales;
@@ -307,6 +310,11 @@ E4m3Params params_of(const GemmE4m3Desc& g, int* err) {
   p.act = g.act;
   p.wide = ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.resid) |
              static_cast<uintptr_t>(2) * g.N) & 15u) == 0;
+  // A residual read by words is waited for row by row, so it is fetched to L2 ahead (4750 x
+  // 260 x 6795: 124 us without, 105 with). Read by vectors it gains where K is short and
+  // the residual and the output do not fit L2 together (4750 x 260 x 6800: 51 and 44 us),
+  // and costs 1 to 5 % elsewhere (4096 x 2048 x 4096: 37.6 and 39.0 us).
+  p.ahead = !p.wide || (g.K <= 1024 && static_cast<int64_t>(4) * g.M * g.N > kFitsL2);
   p.err = err;
   return p;
 }
@@ -476,26 +484,34 @@ __device__ __forceinline__ void box_load(const E4m3Params& p, uint8_t* box, int6
     for (int i = 0; i < 4; ++i)
       *reinterpret_cast<uint4*>(box + box_at(i * 8 + (lane >> 2), lane & 3)) = u[i];
   } else {
-    // sixteen rows' loads at once, a value each, so that none waits for a branch (4750 x 260
-    // x 6795 with the residual: 129 us with eight rows, 124 with sixteen)
+    // Aligned pairs: a row that starts between two words takes each word from its second
+    // element on, and the element before from the lane before (a row's first one is the lane
+    // of its number's). All 32 rows are loaded at once (4750 x 260 x 6795: 105 us with single
+    // elements, sixteen rows at once, 98 so).
     const int k = lane & 15, left = p.N - n - 2 * k;
+    const unsigned short* base =
+        reinterpret_cast<const unsigned short*>(p.resid) + row0 * p.N + n;
+    const uint32_t first = row0 + lane < p.M && n < p.N ? base[(int64_t)lane * p.N] : 0;
+    uint32_t w[16];
 #pragma unroll
-    for (int i0 = 0; i0 < 16; i0 += 8) {
-      unsigned short lo[8], hi[8];
+    for (int i = 0; i < 16; ++i) {
+      const int r = i * 2 + (lane >> 4);
+      const unsigned short* from = base + (int64_t)r * p.N + 2 * k;
+      const int odd = (int)(reinterpret_cast<uintptr_t>(from) >> 1) & 1;
+      w[i] = 0;
+      if (row0 + r < p.M && left > odd + 1)
+        w[i] = *reinterpret_cast<const uint32_t*>(from + odd);
+      else if (row0 + r < p.M && left == odd + 1)
+        w[i] = from[odd];
+    }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = (i0 + i) * 2 + (lane >> 4);
-        const unsigned short* from = reinterpret_cast<const unsigned short*>(p.resid) +
-                                     (row0 + r) * p.N + n + 2 * k;
-        lo[i] = row0 + r < p.M && left > 0 ? from[0] : 0;
-        hi[i] = row0 + r < p.M && left > 1 ? from[1] : 0;
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = (i0 + i) * 2 + (lane >> 4);
-        *reinterpret_cast<uint32_t*>(box + box_at(r, k >> 2) + (k & 3) * 4) =
-            lo[i] | ((uint32_t)hi[i] << 16);
-      }
+    for (int i = 0; i < 16; ++i) {
+      const int r = i * 2 + (lane >> 4);
+      const bool odd = (reinterpret_cast<uintptr_t>(base + (int64_t)r * p.N) & 2u) != 0;
+      const uint32_t before = __shfl_up_sync(0xffffffffu, w[i], 1, 16) >> 16;
+      const uint32_t own = __shfl_sync(0xffffffffu, first, r);
+      *reinterpret_cast<uint32_t*>(box + box_at(r, k >> 2) + (k & 3) * 4) =
+          odd ? (k ? before : own) | (w[i] << 16) : w[i];
     }
   }
 }
@@ -713,6 +729,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
     };
     read_bias(t.n);
+    // ... and its rows of the residual are fetched to L2 where that pays (p.ahead)
+    auto fetch_resid = [&](uint32_t tm, uint32_t tn) {
+      const int64_t row = (int64_t)tm * 256 + rank * 128 + quarter * 32 + lane;
+      if (row >= p.M) return;
+#pragma unroll
+      for (int c = 0; c < COLS; c += 32) {
+        const int n = (int)tn * BN + half * COLS + c;
+        if (n < p.N)
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(p.resid + row * p.N + n));
+      }
+    };
+    if (RESID && p.ahead) fetch_resid(t.m, t.n);
     uint32_t i = 0;
     for (; t.left; ++i) {
       const int64_t row0 = (int64_t)t.m * 256 + rank * 128 + quarter * 32;
@@ -725,6 +753,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       for (int j = 0; j < COLS / 32; ++j) bias[j * 32 + lane] = next_bias[j];
       __syncwarp();
       if (t.left) read_bias(t.n);
+      if (RESID && p.ahead && t.left) fetch_resid(t.m, t.n);
       if (RESID) box_load(p, box, row0, n0 + (half ? COLS - 32 : 0), lane);
       const bool ok = mbar_wait_cluster(&tfull[i & 1], (i >> 1) & 1, abort_flag, p.err);
       if (!__all_sync(0xffffffffu, ok)) {
