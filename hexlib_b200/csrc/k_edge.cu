@@ -44,9 +44,6 @@ __device__ __forceinline__ float gate_value(float g, int act) {
   return act == HEXLIB_B200_GATE_SILU ? g * s : s;
 }
 
-__device__ __forceinline__ float normed(float v, float2 ms, float w, float b) {
-  return fmaf(__fmul_rn(__fsub_rn(v, ms.x), ms.y), w, b);
-}
 __device__ __forceinline__ float blended(float x_scale, float x, float y_scale, float u) {
   return fmaf(x_scale, x, __fmul_rn(y_scale, u));
 }
@@ -63,10 +60,20 @@ __device__ __forceinline__ float inverse_root(float a) {
 // Sum over the G threads of a row: a warp, or the CTA of G threads through shared
 // memory. The slots rotate, so that one barrier a sum suffices: a slot is written
 // again only three barriers after it was read.
+constexpr int kSumSlot = 16;                         // two sums of 8 warps
 template <int G>
 struct RowSum {
-  float (*red)[8];
+  float (*red)[kSumSlot];
   int slot = 0;
+  static __device__ float of_warps(const float* r) {
+    const float4 a = *reinterpret_cast<const float4*>(r);
+    float v = (a.x + a.y) + (a.z + a.w);
+    if constexpr (G == 256) {
+      const float4 b = *reinterpret_cast<const float4*>(r + 4);
+      v += (b.x + b.y) + (b.z + b.w);
+    }
+    return v;
+  }
   __device__ float operator()(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -75,15 +82,48 @@ struct RowSum {
     slot = (slot + 1) & 3;
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
     __syncthreads();
-    const float4 a = *reinterpret_cast<const float4*>(r);
-    v = (a.x + a.y) + (a.z + a.w);
-    if constexpr (G == 256) {
-      const float4 b = *reinterpret_cast<const float4*>(r + 4);
-      v += (b.x + b.y) + (b.z + b.w);
+    return of_warps(r);
+  }
+  // two sums at once
+  __device__ float2 operator()(float2 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+      v = __fadd2_rn(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o),
+                                    __shfl_xor_sync(0xffffffffu, v.y, o)));
+    if constexpr (G == 32) return v;
+    float* r = red[slot];
+    slot = (slot + 1) & 3;
+    if ((threadIdx.x & 31) == 0) {
+      r[threadIdx.x >> 5] = v.x;
+      r[8 + (threadIdx.x >> 5)] = v.y;
     }
-    return v;
+    __syncthreads();
+    return make_float2(of_warps(r), of_warps(r + 8));
   }
 };
+
+// A layer norm takes the mean off each value before it multiplies: the rounding of
+// mean inv in v inv - mean inv would stay in every value (0.5 in a constant row of 30000 at
+// eps 1e-5, whose norm is its shift alone). What rounding leaves out of the mean is held as
+// `rest` and taken off after it, where the values have become small, (d - rest) inv, and its
+// square off the mean square of the d = v - mean.
+struct Mean {
+  float mean, rest;
+};
+// From a sum that is exact where the mean is far larger than the deviations: up to 8192
+// values of one binade, 11 bits each, add up within 24 bits. The remainder of the division
+// is then all that the mean lacks; the first one corrects the quotient.
+__device__ __forceinline__ Mean mean_of(float s, int C, float per_c) {
+  float m = __fmul_rn(s, per_c);
+  m = fmaf(fmaf(-m, (float)C, s), per_c, m);
+  return Mean{m, __fmul_rn(fmaf(-m, (float)C, s), per_c)};
+}
+// What an inexact sum left out of a mean shows in the sum of the deviations, sums.x; with
+// that of their squares, sums.y: the rest and the variance.
+__device__ __forceinline__ float2 corrected(float2 sums, int C, float per_c) {
+  const float rest = mean_of(sums.x, C, per_c).mean;
+  return make_float2(rest, fmaxf(fmaf(-rest, rest, __fmul_rn(sums.y, per_c)), 0.f));
+}
 
 __device__ __forceinline__ float2 halves(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
@@ -180,26 +220,30 @@ struct Row {
   }
 
   // norm(v) w + b, the moments taken over the whole row (the squared deviations of a
-  // layer norm after its mean). v inv - mean inv is one fused step a pair.
+  // layer norm after its mean). Rows too long for an exact sum take what their mean
+  // lacks from the sum of the deviations instead of the division's remainder.
+  static constexpr bool LONG = G * V * 8 > 8192;
   __device__ __forceinline__ void norm(const float* w, const float* b, int C, float per_c,
                                        bool layer, float eps, RowSum<G>& sum) {
-    float2 ss = both(0.f);
-    float mean = 0.f;
+    float2 ss = both(0.f), ds = both(0.f);
+    Mean m = {0.f, 0.f};
     if (layer) {
       float2 s = both(0.f);
 #pragma unroll
       for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) s = __fadd2_rn(s, v[j][q]);
-      mean = sum(s.x + s.y) * per_c;
+      m = mean_of(sum(s.x + s.y), C, per_c);
 #pragma unroll
       for (int j = 0; j < V; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float2 d = __fadd2_rn(v[j][q], both(-mean));
+          float2 d = __fadd2_rn(v[j][q], both(-m.mean));
           if (col.at(j, WIDE ? 0 : 2 * q) >= C) d.x = 0.f;
           if (col.at(j, WIDE ? 0 : 2 * q + 1) >= C) d.y = 0.f;
+          if (LONG) ds = __fadd2_rn(ds, d);
           ss = __ffma2_rn(d, d, ss);
+          v[j][q] = d;
         }
     } else {
 #pragma unroll
@@ -223,8 +267,16 @@ struct Row {
         col.load(wv, w + col.base, j, C);
       }
     };
-    const float inv = inverse_root(fmaf(sum(ss.x + ss.y), per_c, eps));
-    const float2 shift = both(-__fmul_rn(mean, inv));
+    float ms;
+    if (LONG && layer) {
+      const float2 t = corrected(sum(make_float2(ds.x + ds.y, ss.x + ss.y)), C, per_c);
+      m.rest = t.x;
+      ms = __fadd_rn(t.y, eps);
+    } else {
+      ms = fmaf(-m.rest, m.rest, fmaf(sum(ss.x + ss.y), per_c, eps));
+    }
+    const float inv = inverse_root(ms);
+    const float2 shift = both(-__fmul_rn(m.rest, inv));
     if (b) {
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -321,7 +373,7 @@ constexpr int held_ctas(int G, int V) {       // of an SM: registers for V vecto
 }
 template <int G, int V, bool WIDE, bool E4M3>
 __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(const EdgeDesc d) {
-  __shared__ __align__(16) float red[4][8];
+  __shared__ __align__(16) float red[4][kSumSlot];
   if (E4M3) grid_dependents_may_start();   // the product that follows waits itself
   RowSum<G> sum{red};
   constexpr int ROWS = G == 32 ? held_threads(G) / 32 : 1;
@@ -384,7 +436,7 @@ constexpr int row_ctas(int G, int V) {
 template <int G, int V, bool E4M3>
 __global__ void __launch_bounds__(G, row_ctas(G, V)) edge_row(const EdgeDesc d) {
   extern __shared__ __align__(16) __half rows[];     // x, y, gate of a row
-  __shared__ __align__(16) float red[4][8];
+  __shared__ __align__(16) float red[4][kSumSlot];
   __shared__ uint64_t full;
   __shared__ int abort_flag;
   if (E4M3) grid_dependents_may_start();
@@ -448,25 +500,38 @@ __global__ void __launch_bounds__(G, row_ctas(G, V)) edge_row(const EdgeDesc d) 
 
 // Rows wider than the registers hold: one CTA per row, read again for each pass. A
 // thread reads x' of other threads' columns only after the barriers of the sums.
-__device__ __forceinline__ float2 moments_wide(const __half* v, int C, float per_c, bool layer,
-                                               float eps, RowSum<kThreads>& sum) {
-  float mean = 0.f;
-  if (layer) {
-    float s = 0.f;
-    for (int c = threadIdx.x; c < C; c += kThreads) s += __half2float(v[c]);
-    mean = sum(s) * per_c;
-  }
+struct Moments {
+  float mean, inv, shift;                            // of (v - mean) inv + shift
+};
+__device__ __forceinline__ Moments moments_wide(const __half* v, int C, float per_c, bool layer,
+                                                float eps, RowSum<kThreads>& sum) {
   float ss = 0.f;
+  if (!layer) {
+    for (int c = threadIdx.x; c < C; c += kThreads) {
+      const float d = __half2float(v[c]);
+      ss = fmaf(d, d, ss);
+    }
+    return Moments{0.f, inverse_root(fmaf(sum(ss), per_c, eps)), -0.f};
+  }
+  float s = 0.f, ds = 0.f;
+  for (int c = threadIdx.x; c < C; c += kThreads) s += __half2float(v[c]);
+  const float mean = mean_of(sum(s), C, per_c).mean;
   for (int c = threadIdx.x; c < C; c += kThreads) {
     const float d = __half2float(v[c]) - mean;
+    ds += d;
     ss = fmaf(d, d, ss);
   }
-  return make_float2(mean, inverse_root(fmaf(sum(ss), per_c, eps)));
+  const float2 t = corrected(sum(make_float2(ds, ss)), C, per_c);
+  const float inv = inverse_root(__fadd_rn(t.y, eps));
+  return Moments{mean, inv, -__fmul_rn(t.x, inv)};
+}
+__device__ __forceinline__ float normed(float v, const Moments& m, float w, float b) {
+  return fmaf(fmaf(__fsub_rn(v, m.mean), m.inv, m.shift), w, b);
 }
 
 template <bool E4M3>
 __global__ void __launch_bounds__(kThreads) edge_wide(const EdgeDesc d) {
-  __shared__ __align__(16) float red[4][8];
+  __shared__ __align__(16) float red[4][kSumSlot];
   RowSum<kThreads> sum{red};
   const bool layer = d.norm == HEXLIB_B200_NORM_LAYER;
   const int per_gate = d.gate ? d.R / d.gate_rows : 1;
@@ -477,7 +542,7 @@ __global__ void __launch_bounds__(kThreads) edge_wide(const EdgeDesc d) {
       const __half* y = (const __half*)d.y + r * d.C;
       const __half* gate = (const __half*)d.gate + (r / per_gate) * d.C;
       __half* xo = (__half*)d.x_out + r * d.C;
-      float2 ms = make_float2(0.f, 1.f);
+      Moments ms = {0.f, 1.f, -0.f};
       if (d.post_w) ms = moments_wide(y, d.C, per_c, layer, d.eps, sum);
       for (int c = threadIdx.x; c < d.C; c += kThreads) {
         float u = __half2float(y[c]);
@@ -488,7 +553,7 @@ __global__ void __launch_bounds__(kThreads) edge_wide(const EdgeDesc d) {
       x = xo;
     }
     if (!d.pre_w) continue;
-    const float2 ms = moments_wide(x, d.C, per_c, layer, d.eps, sum);
+    const Moments ms = moments_wide(x, d.C, per_c, layer, d.eps, sum);
     auto h_of = [&](int c) {
       return __float2half_rn(normed(__half2float(x[c]), ms, d.pre_w[c],
                                     d.pre_b ? d.pre_b[c] : 0.f));
