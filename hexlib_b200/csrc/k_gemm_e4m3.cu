@@ -68,7 +68,8 @@ __device__ __forceinline__ float finish(float v, int act) {
 //
 // Launched with programmatic serialization: a CTA may start while the kernel before
 // (the quantization of a, which lets it) is still running. Until that has finished it
-// only sets up and brings its part of w to L2, which is right whoever wrote w last.
+// only sets up and brings its part of w to L2, which is right whoever wrote w last; after
+// it, plain loads: the read-only path is for data that nothing writes while the kernel lives.
 template <int BN>
 struct TileCfg {
   static constexpr int W_BYTES = 128 * kBlockK;
@@ -211,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = lane + 32 * j, n = n0 + r, m = m0 + r;
-        w[j] = n < p.N ? __ldg(p.w_scales + (int64_t)g * p.N + n) : 0x7f7f7f7fu;
-        a[j] = r < BN && m < p.M ? __ldg(p.a_scales + (int64_t)g * p.M + m) : 0x7f7f7f7fu;
+        w[j] = n < p.N ? p.w_scales[(int64_t)g * p.N + n] : 0x7f7f7f7fu;
+        a[j] = r < BN && m < p.M ? p.a_scales[(int64_t)g * p.M + m] : 0x7f7f7f7fu;
       }
       const bool ok = mbar_wait(&sf_empty[u & 1], ((u >> 1) & 1) ^ 1, abort_flag, p.err);
       if (!__all_sync(0xffffffffu, ok)) break;
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         st_cluster_u32(cluster_addr(to, tok >> cols_log2), v[c]);
       }
     } else if (n < p.N) {
-      const float bias = p.bias ? __ldg(p.bias + n) : 0.f;
+      const float bias = p.bias ? p.bias[n] : 0.f;
       const int m = m0 + half * COLS + c0;
       const int64_t o = (int64_t)m * p.N + n;
       float r[CH];
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int cols = BN >> split_log2;               // tokens this CTA finishes
     const int f = threadIdx.x & 127;
     const bool in_n = n0 + f < p.N;
-    const float bias = p.bias && in_n ? __ldg(p.bias + n0 + f) : 0.f;
+    const float bias = p.bias && in_n ? p.bias[n0 + f] : 0.f;
     for (int c = threadIdx.x >> 7; c < cols; c += kThreads / 128) {
       const int m = m0 + rank * cols + c;
       if (m >= p.M || !in_n) continue;
@@ -690,12 +691,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         uint32_t a[4], w[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          a[j] = m0 + 32 * j < p.M ? __ldg(p.a_scales + (int64_t)g * p.M + m0 + 32 * j)
-                                   : 0x7f7f7f7fu;
+          a[j] = m0 + 32 * j < p.M ? p.a_scales[(int64_t)g * p.M + m0 + 32 * j] : 0x7f7f7f7fu;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          w[j] = n0 + 32 * j < p.N ? __ldg(p.w_scales + (int64_t)g * p.N + n0 + 32 * j)
-                                   : 0x7f7f7f7fu;
+          w[j] = n0 + 32 * j < p.N ? p.w_scales[(int64_t)g * p.N + n0 + 32 * j] : 0x7f7f7f7fu;
         const bool ok = mbar_wait_cluster(&sf_empty[b], ph, abort_flag, p.err);
         if (!__all_sync(0xffffffffu, ok)) {
           if (lane == 0) st_cluster_u32(peer_abort, 1);
@@ -725,7 +724,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
       for (int j = 0; j < COLS / 32; ++j) {
         const int n = tn * BN + half * COLS + j * 32 + lane;
-        next_bias[j] = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
+        next_bias[j] = p.bias && n < p.N ? p.bias[n] : 0.f;
       }
     };
     read_bias(t.n);
