@@ -423,14 +423,14 @@ int hexlib_b200_attention_fp16(const void* q, const void* k, const void* v,
 }
 
 // Most rows and columns of the operators below: their tiles and padded widths are ints.
-constexpr int kMostE4m3 = 1 << 30;
+constexpr int kMostExtent = 1 << 30;
 
 // The operators of a transformer block in 8-bit floating point. Their refusals
 // come before the initialisation, so that a refused call needs no device.
 
 int hexlib_b200_quantize_e4m3_fp16(const void* x, void* codes, void* scales, int R, int K,
                                    void* stream) {
-  if (R < 0 || K <= 0 || R > kMostE4m3 || K > kMostE4m3) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (R < 0 || K <= 0 || R > kMostExtent || K > kMostExtent) return HEXLIB_B200_ERR_INVAL_PARAMS;
   if (R == 0) return HEXLIB_B200_OK;
   if (!x || !codes || !scales || misaligned(x, 2) || misaligned(codes, 16) ||
       misaligned(scales, 4))
@@ -441,7 +441,7 @@ int hexlib_b200_quantize_e4m3_fp16(const void* x, void* codes, void* scales, int
 
 int hexlib_b200_quantize_weight_e4m3_fp16(const void* w, void* codes, void* scales, int K, int N,
                                           void* stream) {
-  if (K <= 0 || N <= 0 || K > kMostE4m3 || N > kMostE4m3 || !w || !codes || !scales || misaligned(w, 2) ||
+  if (K <= 0 || N <= 0 || K > kMostExtent || N > kMostExtent || !w || !codes || !scales || misaligned(w, 2) ||
       misaligned(codes, 16) || misaligned(scales, 4))
     return HEXLIB_B200_ERR_INVAL_PARAMS;
   HB_ENTRY_INIT();
@@ -450,7 +450,7 @@ int hexlib_b200_quantize_weight_e4m3_fp16(const void* w, void* codes, void* scal
 
 int hexlib_b200_dequant_e4m3_fp16(const void* codes, const void* scales, void* out, int R, int K,
                                   void* stream) {
-  if (R < 0 || K <= 0 || R > kMostE4m3 || K > kMostE4m3) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  if (R < 0 || K <= 0 || R > kMostExtent || K > kMostExtent) return HEXLIB_B200_ERR_INVAL_PARAMS;
   if (R == 0) return HEXLIB_B200_OK;
   if (!codes || !scales || !out || misaligned(codes, 16) || misaligned(scales, 4) ||
       misaligned(out, 2))
@@ -462,7 +462,7 @@ int hexlib_b200_dequant_e4m3_fp16(const void* codes, const void* scales, void* o
 static int matmul_e4m3(const void* a_codes, const void* a_scales, const void* w_codes,
                        const void* w_scales, const float* bias, const void* r, void* out, int M,
                        int K, int N, int act, void* stream) {
-  if (M < 0 || K <= 0 || N <= 0 || M > kMostE4m3 || K > kMostE4m3 || N > kMostE4m3 || act < 0 ||
+  if (M < 0 || K <= 0 || N <= 0 || M > kMostExtent || K > kMostExtent || N > kMostExtent || act < 0 ||
       act > 2)
     return HEXLIB_B200_ERR_INVAL_PARAMS;
   if (M == 0) return HEXLIB_B200_OK;
@@ -503,7 +503,7 @@ int hexlib_b200_matmul_epilogue_residual_e4m3(const void* a_codes, const void* a
 }
 
 static int edge(hb::EdgeDesc& d, bool e4m3, void* stream) {
-  if (d.R < 0 || d.C <= 0 || d.R > kMostE4m3 || d.C > kMostE4m3 ||
+  if (d.R < 0 || d.C <= 0 || d.R > kMostExtent || d.C > kMostExtent ||
       (d.norm != HEXLIB_B200_NORM_RMS && d.norm != HEXLIB_B200_NORM_LAYER) ||
       !(d.eps >= 0.f) || d.gate_act < HEXLIB_B200_GATE_NONE || d.gate_act > HEXLIB_B200_GATE_TANH)
     return HEXLIB_B200_ERR_INVAL_PARAMS;
@@ -585,7 +585,8 @@ int hexlib_b200_rope_pos_fp16(const void* x, int64_t x_stride, const int* positi
                               const uint64_t* table, const int* axis, float mscale, void* y,
                               int64_t y_stride, int T, int H, int D, int rot, int layout,
                               void* stream) {
-  if (T < 0 || H <= 0 || D <= 0 || rot <= 0 || (rot & 1) || rot > D || n_axes < 1 || n_axes > 4 ||
+  if (T < 0 || H <= 0 || D <= 0 || T > kMostExtent || H > kMostExtent || D > kMostExtent || rot <= 0 ||
+      (rot & 1) || rot > D || rot > hb::kRopePosMostRot || n_axes < 1 || n_axes > 4 ||
       (layout != HEXLIB_B200_ROPE_HALF && layout != HEXLIB_B200_ROPE_INTERLEAVED) ||
       x_stride < (int64_t)H * D || y_stride < (int64_t)H * D)
     return HEXLIB_B200_ERR_INVAL_PARAMS;

@@ -186,7 +186,9 @@ struct EdgeDesc {
 int edge_kernels_init();
 int launch_edge(const EdgeDesc& d, cudaStream_t s);
 
-// Rotary positions (k_rope_pos.cu).
+// Rotary positions (k_rope_pos.cu): T, H and D up to 2^30, rot up to what the cosines and
+// sines of a token take of shared memory (96 KiB).
+constexpr int kRopePosMostRot = 24576;
 struct RopePosDesc {
   const void* x;
   int64_t x_stride;

@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads) rope_pos_any(const RopePosDesc d, co
   }
 }
 
-constexpr int kMaxPairBytes = 96 * 1024;   // cosines and sines of a tile
+constexpr int kMaxPairBytes = kRopePosMostRot / 2 * sizeof(float2);   // those of a tile of one token
 
 }  // namespace
 
@@ -223,8 +223,8 @@ int launch_rope_pos(const RopePosDesc& desc, cudaStream_t s) {
   if (d.n_axes == 1) d.axis = nullptr;     // every number clamps to 0
   const bool inter = d.layout == HEXLIB_B200_ROPE_INTERLEAVED;
   const uintptr_t bits = reinterpret_cast<uintptr_t>(d.x) | reinterpret_cast<uintptr_t>(d.y) |
-                         static_cast<uintptr_t>(2 * d.x_stride) |
-                         static_cast<uintptr_t>(2 * d.y_stride) | static_cast<uintptr_t>(2 * d.D);
+                         2 * static_cast<uintptr_t>(d.x_stride) |
+                         2 * static_cast<uintptr_t>(d.y_stride) | 2 * static_cast<uintptr_t>(d.D);
   // the widest vector that divides the rows and the rotated part (each half of it)
   const int part = inter ? d.rot : d.rot / 2;
   int w = 8;
@@ -232,7 +232,6 @@ int launch_rope_pos(const RopePosDesc& desc, cudaStream_t s) {
   if (d.D > 4096) w = 1;
   RopeShape sh;
   sh.pairs = d.rot / 2;
-  if ((int64_t)sh.pairs * 8 > kMaxPairBytes) return HEXLIB_B200_ERR_INVAL_PARAMS;
   sh.rot_items = w > 1 ? part / w : sh.pairs;
   sh.copy_w = w;                           // (w divides rot, D and the strides)
   while (w > 1 && sh.copy_w < 8 &&
@@ -250,11 +249,12 @@ int launch_rope_pos(const RopePosDesc& desc, cudaStream_t s) {
   const int64_t tiles = (d.T + tokens - 1) / tokens;
   int64_t split = 296 / tiles, most = (per_token + kThreads - 1) / kThreads;
   if (split > most) split = most;
-  if (split < (d.H + 1023) / 1024) split = (d.H + 1023) / 1024;   // (items in 32 bits)
+  const int64_t least = ((int64_t)d.H + 1023) / 1024;   // (items in 32 bits)
+  if (split < least) split = least;
   if (split > d.H) split = d.H;
   if (split < 1) split = 1;
   sh.heads = (int)((d.H + split - 1) / split);
-  sh.head_split = (d.H + sh.heads - 1) / sh.heads;
+  sh.head_split = (int)(((int64_t)d.H + sh.heads - 1) / sh.heads);
   if (tiles * sh.head_split > 0x7fffffff) return HEXLIB_B200_ERR_INVAL_PARAMS;
   sh.per_item = (uint32_t)(((1ull << 32) + sh.items - 1) / sh.items);
   sh.per_head = (uint32_t)(((1ull << 32) + sh.heads - 1) / sh.heads);

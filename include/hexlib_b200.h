@@ -381,8 +381,8 @@ HEXLIB_B200_API int hexlib_b200_attention_fp16(const void *q, const void *k, con
  * tokens) and then launch nothing, are ordered on `stream`, allocate nothing and
  * may be captured into a CUDA graph. `stream` must belong to the current device; like
  * every per-kernel entry, the first call on a device sets the library up and must
- * not be inside a capture. Rows, columns and K are at most 2^30. A bounded wait that
- * expires is reported by hexlib_b200_stream_status. */
+ * not be inside a capture. Rows, columns, K, tokens, heads and their widths are at most
+ * 2^30. A bounded wait that expires is reported by hexlib_b200_stream_status. */
 
 /* THE E4M3 FORM of a matrix of R rows of K fp16 values. A row is cut into blocks
  * of 128 (the last one padded with zeros). A block's scale is the power of two
