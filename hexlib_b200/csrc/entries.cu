@@ -521,13 +521,18 @@ static int edge(hb::EdgeDesc& d, bool e4m3, void* stream) {
       misaligned(d.post_w, 4) || misaligned(d.post_b, 4) || misaligned(d.h_codes, 16) ||
       misaligned(d.h_scales, 4))
     return HEXLIB_B200_ERR_INVAL_PARAMS;
-  // in place: x_out on x or y, h on y; nothing else shares
-  auto shares = [](const void* p, const void* q) { return p && p == q; };
-  if (shares(d.h, d.x_out) || shares(d.h, d.x) || shares(d.gate, d.x_out) || shares(d.gate, d.h))
+  // in place: x_out on x or y, h on y; no other output shares
+  auto shares = [](const void* p, std::initializer_list<const void*> with) {
+    for (const void* q : with)
+      if (p && p == q) return true;
+    return false;
+  };
+  if (shares(d.h, {d.x, d.x_out}) || shares(d.h_codes, {d.x, d.y, d.x_out, d.h_scales}) ||
+      shares(d.h_scales, {d.x, d.y, d.x_out}))
     return HEXLIB_B200_ERR_INVAL_PARAMS;
-  if (shares(d.h_codes, d.h_scales)) return HEXLIB_B200_ERR_INVAL_PARAMS;
-  for (const void* p : {d.x, d.y, d.gate, static_cast<const void*>(d.x_out)})
-    if (shares(p, d.h_codes) || shares(p, d.h_scales)) return HEXLIB_B200_ERR_INVAL_PARAMS;
+  for (const void* p : {d.gate, (const void*)d.pre_w, (const void*)d.pre_b, (const void*)d.post_w,
+                        (const void*)d.post_b})
+    if (shares(p, {d.x_out, d.h, d.h_codes, d.h_scales})) return HEXLIB_B200_ERR_INVAL_PARAMS;
   HB_ENTRY_INIT();
   d.err = hb::default_error_word();
   return hb::launch_edge(d, as_stream(stream));

@@ -8,7 +8,7 @@ import re
 import pytest
 
 from hexlib_b200 import build
-from test_block_ops_cpu import BAD, OK, P, ROPE, rc, with_
+from test_block_ops_cpu import BAD, EDGE, EDGE8, OK, P, ROPE, rc, with_
 
 SOURCES = {os.path.basename(p): open(p).read() for p in build._sources()}
 
@@ -58,3 +58,16 @@ def test_rope_takes_no_tokens_of_the_largest_heads():
 def test_dequant_refuses_more_than_the_largest_sizes():
     for R, K in ((BIG, 64), (4, BIG), (2 ** 31 - 1, 64), (4, 2 ** 31 - 1)):
         assert rc("dequant_e4m3_fp16", P, P, P, R, K, None) == BAD
+
+
+# every buffer an address of its own
+EDGE_OWN = {**EDGE, **dict(pw=6 * P, pb=7 * P, w=8 * P, b=9 * P)}
+EDGE8_OWN = {**EDGE8, **dict(q=10 * P, sc=11 * P, pw=6 * P, pb=7 * P, w=8 * P, b=9 * P)}
+
+
+@pytest.mark.parametrize("read", ["pw", "pb", "w", "b", "gate"])
+def test_edge_refuses_outputs_on_what_every_row_reads(read):
+    for out in ("xo", "h"):
+        assert rc("norm_gate_residual_fp16", *with_(EDGE_OWN, **{out: EDGE_OWN[read]})) == BAD
+    for out in ("xo", "q", "sc"):
+        assert rc("norm_gate_residual_e4m3", *with_(EDGE8_OWN, **{out: EDGE8_OWN[read]})) == BAD
