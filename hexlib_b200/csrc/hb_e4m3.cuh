@@ -144,31 +144,9 @@ __device__ __forceinline__ void load8(uint32_t (&w)[4], const __half* p, int lef
              (2 * j + 1 < left ? (uint32_t)q[2 * j + 1] << 16 : 0u);
   }
 }
-template <int VEC>
-__device__ __forceinline__ void store8(__half* p, const uint32_t (&w)[4], int left) {
-  if constexpr (VEC == 8) {
-    if (left > 0) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else if constexpr (VEC == 4) {
-#pragma unroll
-    for (int j = 0; j < 4; j += 2)
-      if (2 * j < left) *reinterpret_cast<uint2*>(p + 2 * j) = make_uint2(w[j], w[j + 1]);
-  } else if constexpr (VEC == 2) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (2 * j < left) *reinterpret_cast<uint32_t*>(p + 2 * j) = w[j];
-  } else {
-    unsigned short* q = reinterpret_cast<unsigned short*>(p);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (2 * j < left) q[2 * j] = (unsigned short)w[j];
-      if (2 * j + 1 < left) q[2 * j + 1] = (unsigned short)(w[j] >> 16);
-    }
-  }
-}
-// The widest VEC of rows of C values starting at p (and at q).
-inline int row_vec(int64_t C, const void* p, const void* q = nullptr) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | reinterpret_cast<uintptr_t>(q) |
-                      static_cast<uintptr_t>(2 * C);
+// The widest VEC of rows of C values starting at p.
+inline int row_vec(int64_t C, const void* p) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(2 * C);
   return a % 16 == 0 ? 8 : a % 8 == 0 ? 4 : a % 4 == 0 ? 2 : 1;
 }
 

@@ -125,13 +125,6 @@ __device__ __forceinline__ float2 corrected(float2 sums, int C, float per_c) {
   return make_float2(rest, fmaxf(fmaf(-rest, rest, __fmul_rn(sums.y, per_c)), 0.f));
 }
 
-__device__ __forceinline__ float2 halves(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // The columns of a thread. With rows of whole 16-byte vectors (WIDE), vector j of thread
 // g is columns (j G + g) 8 to + 7, so 16 threads hold a block of 128. Otherwise a WARP
 // holds a block, element i of a lane 32 (i % 4) further, so that scalar accesses of a
@@ -163,7 +156,8 @@ struct Columns {
   }
   __device__ __forceinline__ void store(__half* row, const uint32_t (&w)[4], int j, int C) const {
     if constexpr (WIDE) {
-      store8<8>(row + off(j, 0), w, C - at(j, 0));
+      if (at(j, 0) < C)
+        *reinterpret_cast<uint4*>(row + off(j, 0)) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
       unsigned short* p = reinterpret_cast<unsigned short*>(row);
 #pragma unroll
@@ -196,7 +190,7 @@ struct Columns {
   }
   // a pair with zeros past C, where a vector may end within the row
   __device__ __forceinline__ uint32_t pack_in(float2 f, int j, int q, int C) const {
-    const uint32_t w = pack(f.x, f.y);
+    const uint32_t w = pack_half2(f.x, f.y);
     if constexpr (WIDE) return w;                    // the vector is in or not: see zero_out
     return (at(j, 2 * q) < C ? w & 0xffffu : 0u) | (at(j, 2 * q + 1) < C ? w & 0xffff0000u : 0u);
   }
@@ -216,7 +210,7 @@ struct Row {
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) v[j][q] = halves(w[j][q]);
+      for (int q = 0; q < 4; ++q) v[j][q] = unpack_half2(w[j][q]);
   }
 
   // norm(v) w + b, the moments taken over the whole row (the squared deviations of a
@@ -308,7 +302,7 @@ struct Row {
         uint32_t w[4];
         gate(j, w);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[j][q] = __fmul2_rn(v[j][q], f(halves(w[q])));
+        for (int q = 0; q < 4; ++q) v[j][q] = __fmul2_rn(v[j][q], f(unpack_half2(w[q])));
       }
     };
     if (act == HEXLIB_B200_GATE_NONE) times([](float2 x) { return x; });
@@ -411,7 +405,7 @@ __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(co
       for (int j = 0; j < V; ++j) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          x[j][q] = col.pack_in(__ffma2_rn(both(d.x_scale), halves(x[j][q]),
+          x[j][q] = col.pack_in(__ffma2_rn(both(d.x_scale), unpack_half2(x[j][q]),
                                            __fmul2_rn(both(d.y_scale), v.v[j][q])), j, q, C);
         col.store((__half*)d.x_out + at, x[j], j, C);
         col.zero_out(x[j], j, C);
@@ -485,7 +479,7 @@ __global__ void __launch_bounds__(G, row_ctas(G, V)) edge_row(const EdgeDesc d) 
       for (int j = 0; j < V; ++j) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          x[j][q] = col.pack_in(__ffma2_rn(both(d.x_scale), halves(x[j][q]),
+          x[j][q] = col.pack_in(__ffma2_rn(both(d.x_scale), unpack_half2(x[j][q]),
                                            __fmul2_rn(both(d.y_scale), v.v[j][q])), j, q, C);
         col.store((__half*)d.x_out + at, x[j], j, C);
         col.zero_out(x[j], j, C);

@@ -787,8 +787,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             const uint32_t h[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              v[4 * q + e] = __fadd2_rn(v[4 * q + e],
-                                        __half22float2(*reinterpret_cast<const __half2*>(&h[e])));
+              v[4 * q + e] = __fadd2_rn(v[4 * q + e], unpack_half2(h[e]));
           }
           *slot = make_uint4(pack_half2(v[4 * q].x, v[4 * q].y),
                              pack_half2(v[4 * q + 1].x, v[4 * q + 1].y),

@@ -10,6 +10,7 @@
 #include <cuda_runtime.h>
 #include <math.h>
 
+#include "hb_device.cuh"
 #include "hb_kernels.h"
 
 namespace hb {
@@ -29,14 +30,6 @@ struct RopeShape {
   // word of the product for every i with i * items < 2^32
   uint32_t per_item, per_head;
 };
-
-__device__ __forceinline__ float2 halves(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-__device__ __forceinline__ uint32_t pack(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 
 // The cosine and sine of every pair of a tile of tokens, for all its heads, pair j at
 // (j % P) * n + j / P: the P pairs of an item n apart, so that the threads of a warp,
@@ -143,17 +136,17 @@ __global__ void __launch_bounds__(kThreads) rope_pos_vec(const RopePosDesc d, co
         if constexpr (INTERLEAVED) {
 #pragma unroll
           for (int q = 0; q < W / 2; ++q) {
-            const float2 f = halves(a[q]), k = c[q * sh.rot_items];
-            a[q] = pack(f.x * k.x - f.y * k.y, f.x * k.y + f.y * k.x);
+            const float2 f = unpack_half2(a[q]), k = c[q * sh.rot_items];
+            a[q] = pack_half2(f.x * k.x - f.y * k.y, f.x * k.y + f.y * k.x);
           }
         } else {
           uint32_t(&e)[W / 2] = u[b][VECS - 1];
 #pragma unroll
           for (int q = 0; q < W / 2; ++q) {
-            const float2 fa = halves(a[q]), fb = halves(e[q]);
+            const float2 fa = unpack_half2(a[q]), fb = unpack_half2(e[q]);
             const float2 k0 = c[2 * q * sh.rot_items], k1 = c[(2 * q + 1) * sh.rot_items];
-            a[q] = pack(fa.x * k0.x - fb.x * k0.y, fa.y * k1.x - fb.y * k1.y);
-            e[q] = pack(fa.x * k0.y + fb.x * k0.x, fa.y * k1.y + fb.y * k1.x);
+            a[q] = pack_half2(fa.x * k0.x - fb.x * k0.y, fa.y * k1.x - fb.y * k1.y);
+            e[q] = pack_half2(fa.x * k0.y + fb.x * k0.x, fa.y * k1.y + fb.y * k1.x);
           }
           store_words<W>(y + half, e);
         }
