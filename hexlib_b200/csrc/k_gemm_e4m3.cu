@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
-constexpr int64_t kFitsL2 = 120ll << 20;   // bytes: of 126 MB of L2
+constexpr int64_t kHalfL2 = 64ll << 20;    // bytes
 
 E4m3Params params_of(const GemmE4m3Desc& g, int* err) {
   E4m3Params p = {};
@@ -311,11 +311,15 @@ E4m3Params params_of(const GemmE4m3Desc& g, int* err) {
   p.act = g.act;
   p.wide = ((reinterpret_cast<uintptr_t>(g.out) | reinterpret_cast<uintptr_t>(g.resid) |
              static_cast<uintptr_t>(2) * g.N) & 15u) == 0;
-  // A residual read by words is waited for row by row, so it is fetched to L2 ahead (4750 x
-  // 260 x 6795: 124 us without, 105 with). Read by vectors it gains where K is short and
-  // the residual and the output do not fit L2 together (4750 x 260 x 6800: 51 and 44 us),
-  // and costs 1 to 5 % elsewhere (4096 x 2048 x 4096: 37.6 and 39.0 us).
-  p.ahead = !p.wide || (g.K <= 1024 && static_cast<int64_t>(4) * g.M * g.N > kFitsL2);
+  // Fetching the residual to L2 a tile ahead pays where it is not there yet and K is too short
+  // to hide its way. By vectors, without and with, at K = 128, 1024, 2048: 4750 x 6800 49.0 and
+  // 40.2 us, 54.1 and 49.2, 65.0 and 65.0 (1536: 57.9 and 56.3; 4096: 105.5 and 108.9);
+  // 7680 x 4096 43.3 and 39.9, 48.7 and 48.0, 60.7 and 62.3; 2600 x 6800, 71 MB of residual
+  // and output, 33.9 and 29.1, 38.2 and 34.3, 42.3 and 42.1; 4096 x 4096, 67 MB, 26.3 and
+  // 25.9, 30.9 and 31.1, 35.9 and 37.1; 16384 x 768, 50 MB, 20.7 and 21.3, 25.4 and 25.6,
+  // 30.1 and 30.6. By words, where every row is waited for, it costs nothing at any K:
+  // 4750 x 6795 112 and 108 at 128, 105 and 103 at 1024, 134 and 134 at 4096.
+  p.ahead = !p.wide || (g.K <= 1024 && static_cast<int64_t>(4) * g.M * g.N > kHalfL2);
   p.err = err;
   return p;
 }
@@ -897,6 +901,8 @@ int gemm_e4m3_kernels_init() {
 // 1 token 8.5 us on 16-token tiles split by 4 (16.9 unsplit), for 256 tokens 16.0 on
 // 64-token tiles (22.0 on pairs, 27 split); 1000 x 1000 for 2000 tokens 10.2 on pairs and
 // on 64-token tiles, 2304 x 256 for 4096 tokens 11.4 on pairs.
+// Its counts, 148 SMs and 74 pairs, are the GPU's this is written for; with fewer the choice
+// may be slower, never wrong.
 struct Choice {
   int bn, split_log2;                      // bn = 0: CTA pairs
 };
