@@ -54,7 +54,8 @@ __global__ void __launch_bounds__(kThreads) quantize_e4m3(const __half* __restri
 
 // The form of the transpose of w [K, N]: a CTA turns a block of 128 of K by 32 columns
 // through shared memory, then a warp has a column's block, 4 values to a lane. Done
-// once per weight.
+// once per weight (4096 x 4096: 44 us, bytes alone 7.7; 768 x 2304: 6.8), by two-byte loads
+// and shared-memory columns.
 __global__ void __launch_bounds__(kThreads) quantize_weight_e4m3(const __half* __restrict__ w,
                                                                  uint8_t* __restrict__ codes,
                                                                  uint8_t* __restrict__ scales,
@@ -84,6 +85,9 @@ __global__ void __launch_bounds__(kThreads) quantize_weight_e4m3(const __half* _
   }
 }
 
+// A value to a thread, with the row's division for each: bound by those instructions and by
+// one- and two-byte accesses (8192 x 4096: 151 us, bytes alone 15.4). It shows what a form
+// holds; no product dequantizes.
 __global__ void dequant_e4m3(const uint8_t* __restrict__ codes,
                              const uint8_t* __restrict__ scales, __half* __restrict__ out,
                              int64_t R, int K) {

@@ -422,7 +422,7 @@ __global__ void __launch_bounds__(held_threads(G), held_ctas(G, V)) edge_held(co
 // x, y and the gate of the next row to shared memory while the norm before the next
 // block and the codes of this one are computed, so no warp waits for memory with its
 // registers full, and more of them fit (16384 x 4096 with a sigmoid gate for each element
-// and 8-bit h: 122 us, 5.0 TB/s; 140 with the rows loaded to registers, 134 with 128
+// and 8-bit h: 124 us, 4.9 TB/s; 140 with the rows loaded to registers, 134 with 128
 // threads of four vectors to a row).
 constexpr int row_ctas(int G, int V) {
   return G == 128 ? (V == 2 ? 8 : 6) : V == 2 ? 4 : V <= 4 ? 3 : 1;
@@ -492,8 +492,10 @@ __global__ void __launch_bounds__(G, row_ctas(G, V)) edge_row(const EdgeDesc d) 
   }
 }
 
-// Rows wider than the registers hold: one CTA per row, read again for each pass. A
-// thread reads x' of other threads' columns only after the barriers of the sums.
+// Rows wider than the registers hold: one CTA per row, read again for each pass, an
+// element at a time (2000 x 20000: 229 us for an rms norm alone, 443 with one on both sides
+// and 8-bit h; bytes once would take 49 and 43). A thread reads x' of other threads' columns
+// only after the barriers of the sums.
 struct Moments {
   float mean, inv, shift;                            // of (v - mean) inv + shift
 };

@@ -375,9 +375,12 @@ HEXLIB_B200_API int hexlib_b200_attention_fp16(const void *q, const void *k, con
                                void *stream);
 
 /* ---- 8-bit floating point, block edges, rotary positions -------------------
- * The operators of a language model's transformer block next to the encoder's
- * kernels above (no counterpart in the reference, whose weights are q4_0 and
- * whose only rotation is rope_2d). All of them take an empty batch (no rows, no
+ * Operators of a transformer block beside the encoder's kernels above (no
+ * counterpart in the reference, whose weights are q4_0 and whose only rotation is
+ * rope_2d), as entries alone: no wire kind and no plan uses them. With
+ * hexlib_b200_attention_qkv_fp16 they make an encoder's block: the library has no
+ * causal mask, no shared key and value heads and no key-value cache, and the product's
+ * activations are the two GELUs. All of them take an empty batch (no rows, no
  * tokens) and then launch nothing, are ordered on `stream`, allocate nothing and
  * may be captured into a CUDA graph. `stream` must belong to the current device; like
  * every per-kernel entry, the first call on a device sets the library up and must
@@ -433,8 +436,11 @@ HEXLIB_B200_API int hexlib_b200_matmul_epilogue_residual_e4m3(
  * gate NULL (gate_rows 0) means 1. h is the norm of the stored x'.
  * pre_w NULL with h NULL: x' alone. y NULL (with post_w, gate and x_out NULL):
  * x' = x, h alone -- the norm before the first block.
- * In place: x_out may be x or y, and h may be y. Every other overlap is refused
- * where the pointers are equal and undefined where they are not. */
+ * In place: x_out may be x or y, and h may be y. Every other overlap of an output is
+ * refused where the pointers are equal and undefined where they are not.
+ * The order of a row's sums, and so the last bit of a value, depends on C and on whether
+ * every pointer (h_codes and h_scales aside) and 2 C are multiples of 16; nothing else
+ * changes it. A constant row of a layer norm (eps > 0) gives b. */
 #define HEXLIB_B200_NORM_RMS     0
 #define HEXLIB_B200_NORM_LAYER   1
 #define HEXLIB_B200_GATE_NONE    0   /* f(g) = g           */
@@ -446,7 +452,8 @@ HEXLIB_B200_API int hexlib_b200_norm_gate_residual_fp16(
     int gate_rows, int gate_act, float x_scale, float y_scale, void *x_out, const float *pre_w,
     const float *pre_b, void *h, int R, int C, int norm, float eps, void *stream);
 /* The same with h in its e4m3 form: exactly hexlib_b200_quantize_e4m3_fp16 of the
- * h above, without writing and reading it. h_codes and h_scales overlap nothing. */
+ * h above (of one that starts at a multiple of 16 where the other pointers do), without
+ * writing and reading it. h_codes and h_scales overlap nothing. */
 HEXLIB_B200_API int hexlib_b200_norm_gate_residual_e4m3(
     const void *x, const void *y, const float *post_w, const float *post_b, const void *gate,
     int gate_rows, int gate_act, float x_scale, float y_scale, void *x_out, const float *pre_w,
